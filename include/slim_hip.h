@@ -533,6 +533,60 @@ int slim_linear24_forward_q4(const void* x_bf16, int64_t ldx, int64_t M, int64_t
                              const void* qR_codes, const void* qR_alpha, int64_t r, int qblock, float a_div, void* y_bf16,
                              int64_t ldy, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- 8-bit integer linears ---------------------------------------------------------------------
+ * The reference emulates quantised inputs and weights with dense floating-point products
+ * (slim/quantization/quantization.py:219-263, :266-304); these multiply the integers themselves.
+ * Codes are int8 rows of slim_rows8_ld(K) = K rounded up to a multiple of 128 bytes, zeros behind column K, with one fp32
+ * scale per row: value = code * scale.  dtype: element type of the floating tensors. */
+#define SLIM_DTYPE_F32 0
+#define SLIM_DTYPE_BF16 1
+#define SLIM_DTYPE_F16 2
+int64_t slim_rows8_ld(int64_t K);
+/* codes[r][k] = rint(x[r][k] * (127 / a)), scale[r] = a / 127, a = max |x[r][:]| (fp32 operations, each rounded once).  A row
+ * with a < 2^-100 gets scale 0 and zero codes; a row that holds an infinity or a NaN gets the scale NaN and zero codes.  x: rows
+ * of ldx >= K elements at any element-aligned address; codes 16-byte aligned, ldc >= slim_rows8_ld(K) and a multiple of 16. */
+int slim_quantize_rows8(const void* x, int dtype, int64_t R, int64_t K, int64_t ldx, int8_t* codes, int64_t ldc, float* scale, void* stream);
+/* codes_t[k][n] = codes[n][k] for n < N, 0 up to ldt >= slim_rows8_ld(N): the operand of slim_linear8_backward. */
+int slim_transpose8(const int8_t* codes, int64_t N, int64_t K, int64_t ld, int8_t* codes_t, int64_t ldt, void* stream);
+/* out[m][n] = (sum_k a[m][k] b[n][k]) * sa[m] * sb[n] + bias[n], the sum in whole numbers (K <= 131071), the rest in fp32,
+ * rounded once to the output's type.  bias (of that type) may be NULL.  Columns K .. slim_rows8_ld(K) of a and b are read and must
+ * be zero in one of the two at least. */
+int64_t slim_gemm8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int slim_gemm8_nt(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, const float* sb, int64_t M, int64_t N, int64_t K,
+                  const void* bias, int dtype, void* out, int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream);
+/* y = the rows of x quantised as by slim_quantize_rows8, times the weight's codes [N, slim_rows8_ld(K)] as by slim_gemm8_nt. */
+int64_t slim_linear8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int slim_linear8_forward(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, const int8_t* codes, const float* scale, int64_t N,
+                         const void* bias, void* y, int64_t ldy, void* workspace, int64_t workspace_bytes, void* stream);
+/* dx[m][k] = sum_n dy[m][n] scale[n] codes[n][k], the gradient of slim_linear8_forward with x's quantisation passed straight
+ * through.  codes_t: [K, slim_rows8_ld(N)] from slim_transpose8.  dy * scale is kept per row as integers of 16 bits (24 for
+ * fp32) against the row's maximum: the error of a row is at most sqrt(N / 12) * 2^-15 (2^-23) of the norm of that row.  Rows
+ * that hold an infinity or a NaN give NaN.  N <= 131071. */
+int64_t slim_linear8_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype);
+int slim_linear8_backward(const void* dy, int dtype, int64_t lddy, int64_t M, int64_t N, const int8_t* codes_t, const float* scale, int64_t K,
+                          void* dx, int64_t lddx, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- AdamW over many tensors (the Trainer's optimizer and clipping, slim/fine_tune.py:197-219) ---------------------
+ * params, grads, ...: HOST arrays of `count` device pointers; numel: HOST array.  All tensors of a call have one dtype; a tensor
+ * is numel consecutive elements at any element-aligned address.  The arrays are read before the call returns. */
+/* norm[0] = sqrt(sum over all tensors of g^2), squares and sums in 64 bits, in an order that depends on the sizes only. */
+int64_t slim_grad_norm_workspace_bytes(int count);
+int slim_grad_norm(const void* const* grads, const int64_t* numel, int count, int dtype, float* norm, void* workspace, int64_t workspace_bytes,
+                   void* stream);
+/* pairs of scales of a tensor with 8-bit moments: one per 512 elements */
+int64_t slim_adamw_blocks(int64_t numel);
+/* g' = g * min(1, max_norm / (norm[0] + 1e-6)) (norm NULL: g); m = beta1 m + (1 - beta1) g'; v = beta2 v + (1 - beta2) g'^2;
+ * w = w (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps), in fp32.
+ * scales NULL: exp_avg and exp_avg_sq are fp32.  Otherwise they are codes, e4m3 and e5m2 (the finite formats of the Open Compute
+ * Project), times scales[block][0] and scales[block][1] (fp32, updated): block maximum / 448 and / 57344.  New codes are rounded
+ * up with probability equal to the value's place between its neighbours, with random bits that are a function of seed, the
+ * tensor's ordinal first_index + i, and the position; a positive second moment never gets the code 0; a block that holds an
+ * infinity or a NaN gets the scale NaN.
+ * masters (16-bit parameters only) NULL: w is the parameter.  Otherwise w is masters[i] (fp32), and the parameter its rounding. */
+int slim_adamw_step(void* const* params, const void* const* grads, void* const* exp_avg, void* const* exp_avg_sq, float* const* scales,
+                    float* const* masters, const int64_t* numel, int count, int dtype, int first_index, int64_t step, double lr, double beta1,
+                    double beta2, double eps, double weight_decay, const float* norm, double max_norm, uint32_t seed, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

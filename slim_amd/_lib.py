@@ -9,7 +9,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libslim_hip.so")
 
-vp, i64, i32, f32, u32 = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_uint32
+vp, i64, i32, f32, f64, u32 = C.c_void_p, C.c_int64, C.c_int, C.c_float, C.c_double, C.c_uint32
 
 # name -> (restype, argtypes); mirrors include/slim_hip.h one to one
 PROTOTYPES = {
@@ -120,6 +120,19 @@ PROTOTYPES = {
     "slim_linear24_workspace_bytes": (i64, [i64, i64, i64, i64]),
     "slim_linear24_forward_q4": (i32, [vp, i64, i64, i64, vp, vp, vp, i64, vp, vp, vp, vp, vp, i64, i32, f32, vp, i64, vp, i64, vp]),
     "slim_linear24_forward": (i32, [vp, i64, i64, i64, vp, vp, vp, i64, vp, vp, vp, i64, f32, vp, i64, vp, i64, vp]),
+    "slim_rows8_ld": (i64, [i64]),
+    "slim_quantize_rows8": (i32, [vp, i32, i64, i64, i64, vp, i64, vp, vp]),
+    "slim_transpose8": (i32, [vp, i64, i64, i64, vp, i64, vp]),
+    "slim_gemm8_workspace_bytes": (i64, [i64, i64, i64]),
+    "slim_gemm8_nt": (i32, [vp, i64, vp, vp, i64, vp, i64, i64, i64, vp, i32, vp, i64, vp, i64, vp]),
+    "slim_linear8_workspace_bytes": (i64, [i64, i64, i64]),
+    "slim_linear8_forward": (i32, [vp, i32, i64, i64, i64, vp, vp, i64, vp, vp, i64, vp, i64, vp]),
+    "slim_linear8_backward_workspace_bytes": (i64, [i64, i64, i64, i32]),
+    "slim_linear8_backward": (i32, [vp, i32, i64, i64, i64, vp, vp, i64, vp, i64, vp, i64, vp]),
+    "slim_grad_norm_workspace_bytes": (i64, [i32]),
+    "slim_grad_norm": (i32, [vp, vp, i32, i32, vp, vp, i64, vp]),
+    "slim_adamw_blocks": (i64, [i64]),
+    "slim_adamw_step": (i32, [vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i64, f64, f64, f64, f64, f64, vp, f64, u32, vp]),
 }
 
 ERR_INVALID, ERR_LAUNCH, ERR_UNSUPPORTED, ERR_SOLVER = -1, -2, -3, -4

@@ -1074,3 +1074,257 @@ def linear24_forward_q4(x, vals, meta, sf, N, bias, qL, qR, r, qblock, a_div, ws
     _lib.call("slim_linear24_forward_q4", _p(x), K, M, K, _p(vals), _p(meta), _p(sf), N, _p(bias), _p(qL[0]), _p(qL[1]),
               _p(qR[0]), _p(qR[1]), r, int(qblock), float(a_div), _p(y), N, _p(ws), ws.numel(), _stream())
     return y
+
+
+# ---- linears in 8-bit integers ------------------------------------------------------------------------------
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _call_at(device, name, *args):
+    """_lib.call with `device` current and its current stream as the last argument."""
+    if device.index == torch.cuda.current_device():
+        _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+        return
+    with torch.cuda.device(device):
+        _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+
+
+def _dtype_code(t, name):
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _rows8(t, name):
+    """(2-d tensor with consecutive elements in its rows, element type code); rows may lie further apart than their length."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be on the GPU: slim_amd has no CPU path (got device {t.device})")
+    code = _dtype_code(t, name)
+    if t.dim() != 2 or t.shape[1] == 0:
+        raise ValueError(f"{name} must be a matrix with at least one column, got {tuple(t.shape)}")
+    if t.shape[0] > 1 and (t.stride(1) != 1 or t.stride(0) < t.shape[1]) or t.shape[1] > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t, code
+
+
+def _stride0(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _codes8(t, rows, name):
+    """A contiguous int8 matrix of codes with `rows` rows (any number when None)."""
+    t = _chk(t, torch.int8, name)
+    if t.dim() != 2 or t.shape[0] == 0 or t.shape[1] % 128 or t.shape[1] == 0 or (rows is not None and t.shape[0] != rows):
+        raise ValueError(f"{name} must be [{'rows' if rows is None else rows}, a multiple of 128], got {tuple(t.shape)}")
+    return t
+
+
+def _same_device(first, *rest):
+    for t in rest:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"all tensors must be on one device, got {first.device} and {t.device}")
+
+
+def _pad128(k):
+    return -(-k // 128) * 128
+
+
+def quantize_rows8(x):
+    """(codes int8 [R, K rounded up to 128], scales fp32 [R]) of the rows of x [R, K] (fp32, bf16 or fp16): symmetric codes
+    rint(x * (127 / a)) with a the row's largest magnitude, scale a / 127, zeros behind column K.  A row below 2^-100
+    everywhere gets scale 0; one that holds an infinity or a NaN gets scale NaN.  Tokens of an activation, or output channels
+    of a weight [N, K] (the operand of linear8_forward)."""
+    x, dt = _rows8(x, "x")
+    R, K = x.shape
+    codes = torch.empty(R, _pad128(K), dtype=torch.int8, device=x.device)
+    scale = torch.empty(R, dtype=torch.float32, device=x.device)
+    if R:
+        _call_at(x.device, "slim_quantize_rows8", x.data_ptr(), dt, R, K, _stride0(x), codes.data_ptr(), codes.shape[1], scale.data_ptr())
+    return codes, scale
+
+
+def transpose8(codes, K):
+    """Codes [K, N rounded up to 128] of the transposed matrix of codes [N, K rounded up to 128] (the operand of
+    linear8_backward)."""
+    codes = _codes8(codes, None, "codes")
+    N = codes.shape[0]
+    if _pad128(K) != codes.shape[1]:
+        raise ValueError(f"codes of {K} columns have {_pad128(K)}, got {codes.shape[1]}")
+    out = torch.empty(K, _pad128(N), dtype=torch.int8, device=codes.device)
+    _call_at(codes.device, "slim_transpose8", codes.data_ptr(), N, K, codes.shape[1], out.data_ptr(), out.shape[1])
+    return out
+
+
+def _vector(t, n, dtype, name):
+    t = _chk(t, dtype, name)
+    if t.numel() != n:
+        raise ValueError(f"{name} must hold {n} values, got {tuple(t.shape)}")
+    return t
+
+
+def gemm8_nt(a, sa, b, sb, bias=None, out_dtype=BF16):
+    """out [M, N] = (a @ b.T) * sa[:, None] * sb (+ bias) for codes a [M, Kp], b [N, Kp] with scales sa [M], sb [N] as
+    quantize_rows8 makes them: the sum in whole numbers, the rest in fp32, rounded once to out_dtype."""
+    a, b = _codes8(a, None, "a"), _codes8(b, None, "b")
+    M, Kp = a.shape
+    N = b.shape[0]
+    if b.shape[1] != Kp:
+        raise ValueError(f"a and b must have equally long rows, got {Kp} and {b.shape[1]}")
+    if out_dtype not in _DTYPES:
+        raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+    sa, sb = _vector(sa, M, torch.float32, "sa"), _vector(sb, N, torch.float32, "sb")
+    if bias is not None:
+        bias = _vector(bias, N, out_dtype, "bias")
+    _same_device(a, b, sa, sb, bias)
+    out = torch.empty(M, N, dtype=out_dtype, device=a.device)
+    nb = _lib.query("slim_gemm8_workspace_bytes", M, N, Kp)
+    ws = _ws(nb, a.device)
+    _call_at(a.device, "slim_gemm8_nt", a.data_ptr(), Kp, sa.data_ptr(), b.data_ptr(), Kp, sb.data_ptr(), M, N, Kp, _p(bias), _DTYPES[out_dtype],
+             out.data_ptr(), N, ws.data_ptr(), ws.numel())
+    return out
+
+
+def linear8_forward(x, codes, scale, bias=None):
+    """y [M, N] = x [M, K], quantised token by token (quantize_rows8), times the weight kept as codes [N, Kp] and scale [N],
+    plus bias [N]; y and bias have the type of x (fp32, bf16 or fp16)."""
+    x, dt = _rows8(x, "x")
+    M, K = x.shape
+    codes = _codes8(codes, None, "codes")
+    N = codes.shape[0]
+    if codes.shape[1] != _pad128(K):
+        raise ValueError(f"codes of a weight with {K} input channels have {_pad128(K)} columns, got {codes.shape[1]}")
+    scale = _vector(scale, N, torch.float32, "scale")
+    if bias is not None:
+        bias = _vector(bias, N, x.dtype, "bias")
+    _same_device(x, codes, scale, bias)
+    y = torch.empty(M, N, dtype=x.dtype, device=x.device)
+    if M:
+        ws = _ws(_lib.query("slim_linear8_workspace_bytes", M, N, K), x.device)
+        _call_at(x.device, "slim_linear8_forward", x.data_ptr(), dt, _stride0(x), M, K, codes.data_ptr(), scale.data_ptr(), N, _p(bias), y.data_ptr(), N,
+                 ws.data_ptr(), ws.numel())
+    return y
+
+
+def linear8_backward(dy, codes_t, scale):
+    """dx [M, K] = (dy [M, N] * scale) @ codes: the gradient of linear8_forward with respect to x, the quantisation of x passed
+    straight through.  codes_t [K, Np] from transpose8; dx has the type of dy.  dy * scale is kept as integers of 16 bits per row
+    (24 for fp32), so a row's error is below sqrt(N / 12) 2^-15 (2^-23) of its norm."""
+    dy, dt = _rows8(dy, "dy")
+    M, N = dy.shape
+    codes_t = _codes8(codes_t, None, "codes_t")
+    K = codes_t.shape[0]
+    if codes_t.shape[1] != _pad128(N):
+        raise ValueError(f"codes_t of a weight with {N} output channels has {_pad128(N)} columns, got {codes_t.shape[1]}")
+    scale = _vector(scale, N, torch.float32, "scale")
+    _same_device(dy, codes_t, scale)
+    dx = torch.empty(M, K, dtype=dy.dtype, device=dy.device)
+    if M:
+        ws = _ws(_lib.query("slim_linear8_backward_workspace_bytes", M, N, K, dt), dy.device)
+        _call_at(dy.device, "slim_linear8_backward", dy.data_ptr(), dt, _stride0(dy), M, N, codes_t.data_ptr(), scale.data_ptr(), K, dx.data_ptr(), K,
+                 ws.data_ptr(), ws.numel())
+    return dx
+
+
+# ---- AdamW over many tensors ----------------------------------------------------------------------------------
+ADAMW_BLOCK = 512         # elements of a tensor that share a pair of scales (8-bit moments)
+
+
+def _dense(t, name):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be on the GPU: slim_amd has no CPU path (got device {t.device})")
+    if t.layout != torch.strided:
+        raise TypeError(f"{name} must be a dense tensor, got {t.layout}")
+
+
+def _addresses(tensors):
+    import ctypes
+    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+def _sizes(tensors):
+    import ctypes
+    return (ctypes.c_int64 * len(tensors))(*[t.numel() for t in tensors])
+
+
+def grad_norm(grads):
+    """sqrt of the sum of squares over all tensors of a list (one element type, one device): a 0-d fp32 tensor, squares and
+    sums in 64 bits.  Empty tensors count nothing; an empty list is refused."""
+    import ctypes
+    grads = list(grads)
+    if not grads:
+        raise ValueError("grad_norm needs at least one tensor")
+    for g in grads:
+        _dense(g, "grads")
+        if g.dtype != grads[0].dtype or g.device != grads[0].device:
+            raise ValueError("grads must have one element type and one device")
+    dt, dev = _dtype_code(grads[0], "grads"), grads[0].device
+    full = [g if g.is_contiguous() else g.contiguous() for g in grads if g.numel()]
+    if not full:
+        return torch.zeros((), dtype=torch.float32, device=dev)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    ws = _ws(_lib.query("slim_grad_norm_workspace_bytes", len(full)), dev)
+    ptrs, sizes = _addresses(full), _sizes(full)
+    _call_at(dev, "slim_grad_norm", ctypes.addressof(ptrs), ctypes.addressof(sizes), len(full), dt, norm.data_ptr(), ws.data_ptr(), ws.numel())
+    return norm
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0, scales=None, masters=None,
+               seed=0, norm=None, max_norm=None, first_index=0):
+    """One AdamW update (slim_adamw_step) of a list of tensors, in place, in one launch per sixty tensors.
+
+    params, grads: lists of contiguous tensors of one element type (fp32, bf16, fp16).  Moments: fp32 tensors of the same sizes, or, with
+    `scales` (fp32 [ceil(n / 512), 2] each), float8_e4m3fn first and float8_e5m2 second moments, rounded stochastically with
+    random bits that are a function of `seed`, the tensor's place first_index + i in the list and the position in it.  masters: fp32 copies
+    of 16-bit parameters, which are then their roundings.  norm (0-d fp32 tensor, grad_norm) with max_norm: the gradients are
+    multiplied by min(1, max_norm / (norm + 1e-6)) as they are read.  step counts from 1.  Empty tensors are left alone.  A captured call
+    replays with the step, lr and seed that it was captured with."""
+    import ctypes
+    lists = [list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), None if scales is None else list(scales), None if masters is None else list(masters)]
+    params, grads, ms, vs, ss, ws = lists
+    count = len(params)
+    if any(x is not None and len(x) != count for x in lists):
+        raise ValueError("adamw_step: all lists must be equally long")
+    if not count:
+        return
+    dtype, dev = params[0].dtype, params[0].device
+    dt = _dtype_code(params[0], "params")
+    moments = (torch.float32, torch.float32) if ss is None else (torch.float8_e4m3fn, torch.float8_e5m2)
+    if ws is not None and dtype == torch.float32:
+        raise ValueError("adamw_step: fp32 parameters need no master copies")
+    if (norm is None) != (max_norm is None):
+        raise ValueError("adamw_step: norm and max_norm go together")
+    checks = [(params, dtype, "params"), (grads, dtype, "grads"), (ms, moments[0], "exp_avgs"), (vs, moments[1], "exp_avg_sqs")]
+    if ws is not None:
+        checks.append((ws, torch.float32, "masters"))
+    sizes = [p.numel() for p in params]
+    for tensors, want, name in checks:
+        for t, n in zip(tensors, sizes):
+            _dense(t, name)
+            if t.dtype != want or t.device != dev or t.numel() != n or not t.is_contiguous():
+                raise ValueError(f"adamw_step: {name} must be contiguous {want} tensors on {dev} of the parameters' sizes")
+    if ss is not None:
+        for s, n in zip(ss, sizes):
+            _dense(s, "scales")
+            if s.dtype != torch.float32 or s.device != dev or tuple(s.shape) != (-(-n // ADAMW_BLOCK), 2) or not s.is_contiguous():
+                raise ValueError(f"adamw_step: scales must be contiguous fp32 [ceil(n / {ADAMW_BLOCK}), 2] tensors on {dev}")
+    if norm is not None:
+        _dense(norm, "norm")
+        if norm.dtype != torch.float32 or norm.numel() != 1 or norm.device != dev:
+            raise ValueError("adamw_step: norm must be one fp32 value on the parameters' device")
+    if 0 in sizes:
+        keep = [i for i, n in enumerate(sizes) if n]
+        params, grads, ms, vs, ss, ws = (None if x is None else [x[i] for i in keep] for x in (params, grads, ms, vs, ss, ws))
+        if not keep:
+            return
+    arrays = [None if x is None else _addresses(x) for x in (params, grads, ms, vs, ss, ws)]
+    numel = _sizes(params)
+    _call_at(dev, "slim_adamw_step", *[None if x is None else ctypes.addressof(x) for x in arrays], ctypes.addressof(numel), len(params), dt,
+             int(first_index), int(step), float(lr), float(beta1), float(beta2), float(eps), float(weight_decay), _p(norm),
+             0.0 if max_norm is None else float(max_norm), int(seed) & 0xffffffff)
+    for p in params:
+        torch.autograd.graph.increment_version(p)
