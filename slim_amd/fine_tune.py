@@ -19,6 +19,8 @@ from itertools import chain
 
 import torch
 
+from .optim import AdamW as SlimAdamW
+
 KNOWN_MODULES = {"Linear", "Conv1d"}
 # the Trainer defaults behind the reference's TrainingArguments (fine_tune.py:197-219)
 LEARNING_RATE = 5e-5
@@ -52,8 +54,11 @@ def disable_linear_layer_grads(model):
     """fine_tune.py:24-48.  Linear / Conv1d modules with adapters: weight and bias frozen (as fp16 only with
     FROZEN_WEIGHT_FP16), pruned adapters (lora_left_mask) re-zeroed before every forward.  Modules without adapters: the
     weight stays trainable under the mask of its current zeros; a tiled-quantised weight (scaling_factor None) is refused.
-    The mask lives on the weight's device (the reference keeps it on the CPU and indexes the device tensor with it)."""
+    The mask lives on the weight's device (the reference keeps it on the CPU and indexes the device tensor with it).
+    Int8Linear modules (slim_amd.packed) hold no trainable weight; their pruned adapters are re-zeroed the same way."""
     for _, module in model.named_modules():
+        if type(module).__name__ == "Int8Linear" and hasattr(module, "lora_left_mask"):
+            module.register_forward_pre_hook(_mask_lora)
         if type(module).__name__ not in KNOWN_MODULES:
             continue
         if hasattr(module, "lora_left"):
@@ -149,7 +154,15 @@ def get_token_blocks(tokenizer, dataset_name="c4", dataset_config_name=None, val
 
 
 def make_optimizer(name, params):
-    """The `optim` names of the Trainer this build covers."""
+    """The `optim` names of the Trainer this build covers, and "adamw_slim": the library's own AdamW with 32-bit moments and
+    32-bit copies of 16-bit parameters (their updates are otherwise lost to the parameters' rounding).  The 8-bit names keep the moments
+    in 8 bits.  Both clip the gradients themselves, while they read them."""
+    if name == "adamw_slim":
+        return SlimAdamW(params, lr=LEARNING_RATE, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, master_weights=True,
+                         max_grad_norm=MAX_GRAD_NORM, seed=SEED)
+    if name in ("adamw_8bit", "adamw_bnb_8bit"):
+        return SlimAdamW(params, lr=LEARNING_RATE, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, state_bits=8,
+                         max_grad_norm=MAX_GRAD_NORM, seed=SEED)
     if name in ("adamw_torch", "adamw_hf", "adamw_torch_fused"):
         return torch.optim.AdamW(params, lr=LEARNING_RATE, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0,
                                  fused=(name == "adamw_torch_fused") or None)
@@ -273,7 +286,8 @@ def fine_tune(model, tokenizer, dataset_name="c4", dataset_config_name=None, val
             running += float(loss.detach())
         if world > 1:
             all_reduce_grads(params, world)
-        torch.nn.utils.clip_grad_norm_(params, MAX_GRAD_NORM)
+        if not isinstance(opt, SlimAdamW):
+            torch.nn.utils.clip_grad_norm_(params, MAX_GRAD_NORM)
         opt.step()
         opt.zero_grad(set_to_none=True)
         since += 1

@@ -1165,9 +1165,10 @@ def _vector(t, n, dtype, name):
     return t
 
 
-def gemm8_nt(a, sa, b, sb, bias=None, out_dtype=BF16):
+def gemm8_nt(a, sa, b, sb, bias=None, out_dtype=BF16, K=None):
     """out [M, N] = (a @ b.T) * sa[:, None] * sb (+ bias) for codes a [M, Kp], b [N, Kp] with scales sa [M], sb [N] as
-    quantize_rows8 makes them: the sum in whole numbers, the rest in fp32, rounded once to out_dtype."""
+    quantize_rows8 makes them: the sum in whole numbers, the rest in fp32, rounded once to out_dtype.  K: the number of columns
+    that are not padding (all when None), at most 131071."""
     a, b = _codes8(a, None, "a"), _codes8(b, None, "b")
     M, Kp = a.shape
     N = b.shape[0]
@@ -1175,14 +1176,17 @@ def gemm8_nt(a, sa, b, sb, bias=None, out_dtype=BF16):
         raise ValueError(f"a and b must have equally long rows, got {Kp} and {b.shape[1]}")
     if out_dtype not in _DTYPES:
         raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
+    K = Kp if K is None else int(K)
+    if not Kp - 128 < K <= Kp:
+        raise ValueError(f"gemm8_nt: K must lie in ({Kp - 128}, {Kp}], got {K}")
     sa, sb = _vector(sa, M, torch.float32, "sa"), _vector(sb, N, torch.float32, "sb")
     if bias is not None:
         bias = _vector(bias, N, out_dtype, "bias")
     _same_device(a, b, sa, sb, bias)
     out = torch.empty(M, N, dtype=out_dtype, device=a.device)
-    nb = _lib.query("slim_gemm8_workspace_bytes", M, N, Kp)
+    nb = _lib.query("slim_gemm8_workspace_bytes", M, N, K)
     ws = _ws(nb, a.device)
-    _call_at(a.device, "slim_gemm8_nt", a.data_ptr(), Kp, sa.data_ptr(), b.data_ptr(), Kp, sb.data_ptr(), M, N, Kp, _p(bias), _DTYPES[out_dtype],
+    _call_at(a.device, "slim_gemm8_nt", a.data_ptr(), Kp, sa.data_ptr(), b.data_ptr(), Kp, sb.data_ptr(), M, N, K, _p(bias), _DTYPES[out_dtype],
              out.data_ptr(), N, ws.data_ptr(), ws.numel())
     return out
 

@@ -1,7 +1,12 @@
 """Inference from packed storage: a compressed nn.Linear (2:4 sparse 4-bit weight + low-rank adapters, as
 slim.prune.prune_and_quantize / slim.lora.quantize_lora leave it) is replaced by a module that keeps the
 weight at 0.375 byte per element and runs Linear + adapter hook (reference slim/prune.py:303-321) as two
-fused launches.  The reference itself only emulates this forward with dense bf16 tensors."""
+fused launches.  The reference itself only emulates this forward with dense bf16 tensors.
+
+Int8Linear is the 8-bit counterpart, for linears with any pattern of zeros: the weight as int8 codes with one scale per
+output channel, the input quantised token by token, the product in whole numbers (the reference emulates it with fake-quantised
+bf16 tensors, slim/quantization/quantization.py:219-263, :266-304).  Its adapters stay what they were, and it passes gradients
+to its input, so the adapters can be fine-tuned over the frozen 8-bit weight (slim_amd.fine_tune)."""
 import math
 
 import torch
@@ -148,9 +153,139 @@ class PackedLinear(torch.nn.Module):
         return f"in_features={self.in_features}, out_features={self.out_features}, rank={self.rank}, packed 2:4 int4"
 
 
-def pack_model(model):
-    """Replace every compressed Linear of the decoder blocks by a PackedLinear, in place.  Returns
-    (dense bytes, packed bytes) of the replaced layers."""
+class _Int8Product(torch.autograd.Function):
+    """The product of Int8Linear; its gradient passes the quantisation of the input straight through (as the reference's
+    QuantizedMatmul does with the weight's, quantization.py:322-328).  The weight and bias are frozen."""
+
+    @staticmethod
+    def forward(ctx, x, module):
+        ctx.module = module
+        return module.product(x)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return ops.linear8_backward(dy, ctx.module.transposed(), ctx.module.scale), None
+
+
+class Int8Linear(torch.nn.Module):
+    """Drop-in for an nn.Linear in 8-bit integers, for inference and for fine-tuning adapters over it.
+
+    A weight that lies on a per-tensor grid of at most 8 bits (what prune_and_quantize leaves: values code / scaling_factor) keeps
+    its codes exactly; any other weight is quantised here, one scale per output channel (ops.quantize_rows8).  The activation
+    is quantised token by token on every call.  Adapters (lora_left, lora_right, lora_rank, lora_quantizer, lora_left_mask) and
+    forward hooks of the linear carry over; its input fake-quantisation pre-hooks do not (the input is quantised here).
+    As with PackedLinear the tensors are plain attributes: `model.to(dtype)` does not change them."""
+
+    TENSORS = ("codes", "scale", "bias", "lora_left", "lora_right", "lora_left_mask")
+
+    def __init__(self, lin=None):
+        super().__init__()
+        self._codes_t = None
+        if lin is None:              # filled by from_tensors
+            return
+        W = lin.weight.data
+        if not W.is_cuda:
+            raise RuntimeError("Int8Linear needs a weight on the GPU (slim_amd has no CPU path)")
+        self.out_features, self.in_features = W.shape
+        self.codes, self.scale = self._codes_of(W, getattr(lin, "scaling_factor", None))
+        self.bias = None if lin.bias is None else lin.bias.data.contiguous()
+        for name in ("lora_left", "lora_right", "lora_rank", "lora_quantizer", "lora_left_mask"):
+            if hasattr(lin, name):
+                setattr(self, name, getattr(lin, name))
+        for hook_id, hook in lin._forward_hooks.items():
+            self._forward_hooks[hook_id] = hook
+
+    @staticmethod
+    def _codes_of(W, sf):
+        """(codes, scale): the grid of a per-tensor scaling factor where every value lies on it (one synchronisation), else
+        quantised rows."""
+        if sf is not None and sf.numel() == 1:
+            sf = sf.detach().to(device=W.device, dtype=torch.float32).reshape(())
+            c = torch.round(W.float() * sf)
+            if bool(((c / sf).to(W.dtype) == W).all() & (c.amin() >= -128) & (c.amax() <= 127)):
+                codes = torch.zeros(W.shape[0], -(-W.shape[1] // 128) * 128, dtype=torch.int8, device=W.device)
+                codes[:, :W.shape[1]] = c.to(torch.int8)
+                return codes, (1.0 / sf).expand(W.shape[0]).contiguous()
+        return ops.quantize_rows8(W)
+
+    @classmethod
+    def from_tensors(cls, tensors, out_features, in_features, device, rank=None, quantizer=None):
+        """Rebuild from the tensors `state()` returns (a checkpoint written by save_packed)."""
+        from .prune import add_lora_hook
+        from .quantization.quantization import Quantizer
+        self = cls()
+        self.out_features, self.in_features = int(out_features), int(in_features)
+        got = {k: (None if tensors.get(k) is None else tensors[k].to(device).contiguous()) for k in cls.TENSORS}
+        self.codes, self.scale, self.bias = got["codes"], got["scale"], got["bias"]
+        if tuple(self.codes.shape) != (self.out_features, -(-self.in_features // 128) * 128) or self.scale.numel() != self.out_features:
+            raise ValueError("8-bit tensors do not match the recorded shape")
+        if got["lora_left"] is not None:
+            self.lora_left, self.lora_right = torch.nn.Parameter(got["lora_left"]), torch.nn.Parameter(got["lora_right"])
+            self.lora_rank = torch.tensor(rank)
+            if got["lora_left_mask"] is not None:
+                self.lora_left_mask = got["lora_left_mask"]
+            if quantizer is not None:
+                self.lora_quantizer = Quantizer("weight", **quantizer)
+            self.register_forward_hook(add_lora_hook)
+        return self
+
+    def state(self):
+        return {k: getattr(self, k).data for k in self.TENSORS if getattr(self, k, None) is not None}
+
+    def info(self):
+        """What from_tensors needs beside the tensors (plain values)."""
+        out = dict(out_features=self.out_features, in_features=self.in_features)
+        if hasattr(self, "lora_left"):
+            out["rank"] = int(self.lora_rank)
+            q = getattr(self, "lora_quantizer", None)
+            if q is not None:
+                out["quantizer"] = dict(num_bits=q.num_bits, slim_quant=q.slim_quant, block_quantization=q.block_quantization, block_dim=q.block_dim)
+        return out
+
+    def packed_bytes(self):
+        """Bytes of codes and scales, and of the adapters where there are any."""
+        return sum(t.numel() * t.element_size() for k, t in self.state().items() if k != "lora_left_mask")
+
+    def dense_weight(self):
+        """The weight the codes stand for, fp32 [N, K]."""
+        return self.codes[:, :self.in_features].float() * self.scale[:, None]
+
+    def transposed(self):
+        """The codes in the order of the backward pass, laid out on its first use and kept (as large as the codes)."""
+        if self._codes_t is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("Int8Linear: the first backward pass lays out the transposed codes and cannot be captured; run one eagerly, "
+                                   "or call transposed() before the capture")
+            self._codes_t = ops.transpose8(self.codes, self.in_features)
+            torch.cuda.current_stream(self.codes.device).synchronize()       # (whatever stream uses them next)
+        return self._codes_t
+
+    def product(self, x2):
+        bias = self.bias
+        if bias is not None and bias.dtype != x2.dtype:
+            bias = bias.to(x2.dtype)
+        return ops.linear8_forward(x2, self.codes, self.scale, bias)
+
+    def forward(self, x):
+        if x.shape[-1] != self.in_features:
+            raise ValueError(f"Int8Linear: the input has {x.shape[-1]} channels, the weight {self.in_features}")
+        if torch.is_autocast_enabled("cuda") and x.dtype == torch.float32:
+            x = x.to(torch.get_autocast_dtype("cuda"))
+        x2 = x.reshape(-1, self.in_features)
+        y = _Int8Product.apply(x2, self) if torch.is_grad_enabled() and x2.requires_grad else self.product(x2)
+        return y.reshape(*x.shape[:-1], self.out_features)
+
+    def extra_repr(self):
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, int8"
+
+
+def pack_model(model, form="2:4"):
+    """Replace every Linear of the decoder blocks in place: by a PackedLinear (form "2:4": compressed to 2:4 int4), or by
+    an Int8Linear (form "int8": any weight).  Returns (dense bytes, packed bytes) of the replaced layers."""
+    kinds = {"2:4": PackedLinear, "int8": Int8Linear}
+    if form not in kinds:
+        raise ValueError(f"form must be one of {sorted(kinds)}, got {form!r}")
     dense = packed = 0
     for layer in get_layers_list(model):
         subset = find_layers(layer)
@@ -159,7 +294,7 @@ def pack_model(model):
             parts = name.split(".")
             for p in parts[:-1]:
                 parent = getattr(parent, p)
-            pl = PackedLinear(lin)
+            pl = kinds[form](lin)
             setattr(parent, parts[-1], pl)
             dense += lin.weight.numel() * 2
             packed += pl.packed_bytes()
@@ -167,19 +302,21 @@ def pack_model(model):
 
 
 FORMAT = "slim_amd.packed24/1"
+FORMAT_INT8 = "slim_amd.int8/1"
 
 
-def _packed_modules(model):
+def _packed_modules(model, kind=PackedLinear):
     for i, layer in enumerate(get_layers_list(model)):
         for name, mod in layer.named_modules():
-            if isinstance(mod, PackedLinear):
+            if isinstance(mod, kind):
                 yield f"{i}.{name}", layer, name, mod
 
 
 def save_packed(model, path):
     """Write every PackedLinear of `model` to one safetensors file: per layer `<block>.<name>.{vals,meta,sf,bias,
-    LeffT,ReffT}` plus the shapes, rank and activation divisor in the file's metadata.  The rest of the model
-    (embeddings, norms, head) is not touched -- save it the usual way."""
+    LeffT,ReffT}` plus the shapes, rank and activation divisor in the file's metadata; or every Int8Linear:
+    `<block>.<name>.{codes,scale,bias,lora_left,lora_right,lora_left_mask}`.  A model that holds both is refused.  The rest of
+    the model (embeddings, norms, head) is not touched -- save it the usual way."""
     import json
     from safetensors.torch import save_file
     tensors, index = {}, {}
@@ -188,30 +325,38 @@ def save_packed(model, path):
             tensors[f"{key}.{k}"] = t.detach().cpu().contiguous()
         index[key] = dict(out_features=mod.out_features, in_features=mod.in_features, rank=mod.rank, a_div=mod.a_div,
                           qblock=mod.qblock)
+    int8 = list(_packed_modules(model, Int8Linear))
+    if index and int8:
+        raise ValueError("the model holds both PackedLinear and Int8Linear layers; a file holds one kind")
+    for key, _, _, mod in int8:
+        for k, t in mod.state().items():
+            tensors[f"{key}.{k}"] = t.detach().cpu().contiguous()
+        index[key] = mod.info()
     if not index:
-        raise ValueError("the model holds no PackedLinear; call pack_model first")
-    save_file(tensors, path, metadata={"format": FORMAT, "layers": json.dumps(index)})
+        raise ValueError("the model holds no PackedLinear or Int8Linear; call pack_model first")
+    save_file(tensors, path, metadata={"format": FORMAT_INT8 if int8 else FORMAT, "layers": json.dumps(index)})
     return index
 
 
 def load_packed(model, path, device="cuda"):
-    """Replace the linears named in a save_packed file by PackedLinear modules built from it (the model needs the
-    right architecture, not the right weights).  Returns the number of layers replaced."""
+    """Replace the linears named in a save_packed file by PackedLinear (or Int8Linear) modules built from it (the model
+    needs the right architecture, not the right weights).  Returns the number of layers replaced."""
     import json
     from safetensors import safe_open
     with safe_open(path, framework="pt", device="cpu") as f:
         meta = f.metadata() or {}
-        if meta.get("format") != FORMAT:
-            raise ValueError(f"{path} is not a {FORMAT} file")
+        kind = {FORMAT: PackedLinear, FORMAT_INT8: Int8Linear}.get(meta.get("format"))
+        if kind is None:
+            raise ValueError(f"{path} is not a {FORMAT} or {FORMAT_INT8} file")
         index = json.loads(meta["layers"])
         names = set(f.keys())
         layers = get_layers_list(model)
         for key, info in index.items():
             block, name = key.split(".", 1)
-            tensors = {k: f.get_tensor(f"{key}.{k}") for k in PackedLinear.TENSORS if f"{key}.{k}" in names}
+            tensors = {k: f.get_tensor(f"{key}.{k}") for k in kind.TENSORS if f"{key}.{k}" in names}
             parent = layers[int(block)]
             parts = name.split(".")
             for p in parts[:-1]:
                 parent = getattr(parent, p)
-            setattr(parent, parts[-1], PackedLinear.from_tensors(tensors, device=device, **info))
+            setattr(parent, parts[-1], kind.from_tensors(tensors, device=device, **info))
     return len(index)
