@@ -167,17 +167,21 @@ def load():
     return lib
 
 
+def raise_status(name, rc):
+    """Raise for a non-zero status of an int-returning entry point."""
+    msg = load().slim_last_error().decode(errors="replace")
+    if rc == ERR_UNSUPPORTED:
+        raise NotImplementedError(f"{name}: {msg}")
+    if rc == ERR_INVALID:
+        raise ValueError(f"{name}: {msg}")
+    raise SlimHipError(name, rc, msg)
+
+
 def call(name, *args):
     """Call an int-returning entry point; raise on a non-zero status."""
-    lib = load()
-    rc = getattr(lib, name)(*args)
+    rc = getattr(load(), name)(*args)
     if rc != 0:
-        msg = lib.slim_last_error().decode(errors="replace")
-        if rc == ERR_UNSUPPORTED:
-            raise NotImplementedError(f"{name}: {msg}")
-        if rc == ERR_INVALID:
-            raise ValueError(f"{name}: {msg}")
-        raise SlimHipError(name, rc, msg)
+        raise_status(name, rc)
 
 
 def query(name, *args):

@@ -11,6 +11,12 @@ typedef __attribute__((ext_vector_type(4))) int i32x4;
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef const __attribute__((address_space(1))) void* glb_ptr_t;
 
+int64_t pad128(int64_t k) { return (k + 127) / 128 * 128; }
+int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
+int planes_of(int dtype) { return dtype == SLIM_DTYPE_F32 ? 3 : 2; }
+bool known(int dtype) { return dtype == SLIM_DTYPE_F32 || dtype == SLIM_DTYPE_BF16 || dtype == SLIM_DTYPE_F16; }
+int64_t element_size(int dtype) { return dtype == SLIM_DTYPE_F32 ? 4 : 2; }
+
 // ---- element types --------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(bf16_t v) { return bf16_to_f32(v); }
@@ -45,6 +51,17 @@ template <int PLANES>
 struct Levels {
     static constexpr float value = PLANES == 1 ? 127.f : PLANES == 2 ? 32639.f : 8355711.f;
 };
+
+struct RowScale {
+    float scale, inverse;
+    bool none;                                           // nothing to keep, or nothing that could be kept
+};
+template <int PLANES>
+__device__ __forceinline__ RowScale row_scale(uint32_t max_bits) {
+    const float a = __uint_as_float(max_bits);
+    const bool bad = max_bits >= 0x7f800000u, none = bad || a < 0x1p-100f;
+    return {bad ? __uint_as_float(0x7fc00000u) : none ? 0.f : a / Levels<PLANES>::value, none ? 0.f : Levels<PLANES>::value / a, none};
+}
 
 template <int PLANES>
 __device__ __forceinline__ void store_codes(const float x[8], float r, int8_t* codes, int64_t ldc, int64_t row, int64_t col) {
@@ -128,17 +145,15 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
         __syncthreads();
         m = max(max(part[0], part[1]), max(part[2], part[3]));
     }
-    const float a = __uint_as_float(m);
-    const bool bad = m >= 0x7f800000u, none = bad || a < 0x1p-100f;
-    const float r = none ? 0.f : Levels<PLANES>::value / a;
-    if (t == 0) scale[row] = bad ? __uint_as_float(0x7fc00000u) : none ? 0.f : a / Levels<PLANES>::value;
+    const RowScale rs = row_scale<PLANES>(m);
+    if (t == 0) scale[row] = rs.scale;
     const int64_t end = (K + 127) / 128 * 128;
     auto put = [&](int64_t c, float v[8]) {
-        if (none) {                                      // (x * 0 would be a NaN for what is not finite)
+        if (rs.none) {                                   // (x * 0 would be a NaN for what is not finite)
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = 0.f;
         }
-        store_codes<PLANES>(v, r, codes, ldc, row, c);
+        store_codes<PLANES>(v, rs.inverse, codes, ldc, row, c);
     };
     if (NV > 0) {
 #pragma unroll
@@ -195,6 +210,8 @@ struct Gemm8Args {
     int64_t ldo;
     int dtype;
     int tiles_m, tiles_n;
+    int splits, steps_per_split;                         // slices of the reduction, each into a slab of its own
+    int32_t* slab;                                       // [splits][tiles_m * BM][tiles_n * BN], or null: one slice, results written here
 };
 
 template <int N>
@@ -207,8 +224,13 @@ __device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int dtype
     if (dtype == SLIM_DTYPE_BF16) return bf16_to_f32(((const bf16_t*)p)[i]);
     return (float)((const _Float16*)p)[i];
 }
+__device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float v) {
+    if (dtype == SLIM_DTYPE_F32) ((float*)p)[i] = v;
+    else if (dtype == SLIM_DTYPE_BF16) ((bf16_t*)p)[i] = f32_to_bf16(v);
+    else ((_Float16*)p)[i] = (_Float16)v;
+}
 
-// n (4 .. 32) consecutive results of one row, from any element-aligned address
+// CNT consecutive results of one row, from any element-aligned address
 template <int CNT, typename T, typename F>
 __device__ __forceinline__ void store_row(T* dst, int64_t left, F value) {
     if (left >= CNT) {
@@ -226,23 +248,63 @@ __device__ __forceinline__ void store_row(T* dst, int64_t left, F value) {
     }
 }
 
-// D = A B^T on 16 x 16 x 64 int8 instructions, operands delivered by LDS-DMA (16 bytes per lane) one 128-byte step ahead.
-// LDS image of a stage: BM rows of A, then BN rows of B, 128 bytes each; the 16-byte piece c of a row is stored at c ^ key(row),
-// applied on the source side.  The result is computed transposed (B's fragment as the first operand): a lane then holds
+template <int CNT, typename T>
+__device__ __forceinline__ void load_run(const T* src, int64_t left, float out[CNT]) {
+#pragma unroll
+    for (int c = 0; c < CNT; c += 8) load8(src + c, left - c, out + c);
+}
+
+// One value from its planes' sums, the highest plane first.
+template <int PLANES>
+__device__ __forceinline__ float join_planes(const int* sums, int stride) {
+    float v = (float)sums[0];
+#pragma unroll
+    for (int p = 1; p < PLANES; ++p) v = v * 256.f + (float)sums[p * stride];
+    return v;
+}
+
+// The workgroup's tile and slice.  Workgroups go to the eight XCDs in turn; each XCD gets a run of consecutive tiles, and a run
+// walks groups of eight rows of tiles column by column, so that the 32 workgroups of an XCD share 8 panels of A and 4 of B in
+// its L2 (4096 x 11008 x 4096 on the 256 x 256 tile: 159 us, with groups of four 171 us).
+__device__ __forceinline__ void tile_of(const Gemm8Args& g, int& tm, int& tn, int& slice) {
+    const int per = g.tiles_m * g.tiles_n, total = per * g.splits, b = blockIdx.x, x = b & 7, share = total >> 3, rest = total & 7;
+    const int t = x * share + min(x, rest) + (b >> 3);
+    slice = t / per;
+    const int u = t - slice * per, group = u / (8 * g.tiles_n), m0 = group * 8, gm = min(8, g.tiles_m - m0), r = u - group * 8 * g.tiles_n;
+    tm = m0 + r % gm;
+    tn = r / gm;
+}
+
+// D = A B^T on 16 x 16 x 64 int8 instructions, operands delivered by LDS-DMA (16 bytes per lane) a 128-byte step ahead, two
+// stages.  LDS image of a stage: BM rows of A, then BN rows of B, 128 bytes each; the 16-byte piece c of a row is stored at
+// c ^ key(row), applied on the source side.  The result is computed transposed (B's fragment as the first operand): a lane then holds
 // consecutive columns of one row, and with the rows of B dealt to the fragments in runs of four (row (r / 4) * 4 FN + 4 j + r % 4
 // for lane row r of fragment j) all 4 FN of them are consecutive, so a lane stores its part of a row in 16-byte pieces.
-// key(row) = the lane row's low three bits in either operand, which spreads eight lanes over the eight pieces of a row.
-template <int PLANES, int FM, int FN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void gemm8_kernel(const Gemm8Args g) {
+// key(row) = the lane row's low three bits in either operand, which spreads eight lanes over the eight pieces of a row (no bank
+// conflicts measured).
+// Fragments are double-buffered in registers: while a step's first half (64 bytes) is multiplied its second half is read, and
+// while that is multiplied the next step's first half is read and the stage just emptied is requested again -- one read or request
+// per two matrix instructions, one barrier per step.  Left to the compiler the reads come in a burst that the matrix instructions
+// wait for (4096 x 11008 x 4096, 256 x 256 tile: 185 us against 159; 8192^3: 485 against 397 us, 2.8e15 operations/s).
+// Whole 128-byte lines per row: with 64-byte steps, which would allow four stages, the requests take twice as long (171 us).
+// What bounds it: without requests the loop takes 138 us, without fragment reads as well 123 us; the matrix instructions alone hold
+// the clock at about 2.1 GHz.
+template <int PLANES, int FM, int FN, int WM, int WN, int STAGES, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void gemm8_kernel(const Gemm8Args g) {
     constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN, NW = WM * WN;
-    constexpr int PIECES = (BM + BN) / 8, PPW = (PIECES + NW - 1) / NW;
+    constexpr int PIECES = (BM + BN) / 8, PPW = (PIECES + NW - 1) / NW;     // (a last wave repeats the final piece)
     constexpr int STAGE_BYTES = (BM + BN) * 128;
+    constexpr int RUN = 4 * FN;                          // consecutive columns of a lane
     constexpr int KB = FN == 8 ? 5 : FN == 4 ? 4 : FN == 2 ? 3 : 2;      // the bit of a B row that tells lane rows r and r + 4 apart
+    constexpr int READS = FM + FN, PRODUCTS = FM * FN;
+    constexpr int PACE1 = PRODUCTS / READS > 0 ? PRODUCTS / READS : 1, PACE2 = PRODUCTS / (READS + PPW) > 0 ? PRODUCTS / (READS + PPW) : 1;
     static_assert(FM % PLANES == 0, "a wave holds whole groups of planes");
-    static_assert(BM % 8 == 0 && BN % 8 == 0, "pieces are eight rows");
+    
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int64_t row0 = (int64_t)(blockIdx.x % g.tiles_m) * BM, col0 = (int64_t)(blockIdx.x / g.tiles_m) * BN;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int tm, tn, slice;
+    tile_of(g, tm, tn, slice);
+    const int64_t row0 = (int64_t)tm * BM, col0 = (int64_t)tn * BN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave / WN, wc = wave % WN;
     const int fr = lane & 15, fq = lane >> 4;
 
@@ -252,101 +314,516 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm8_kernel(const Gemm8Args g) 
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
 
-    const int8_t* src[PPW];
-    int dst[PPW];
+    // this lane's sources: row lane / 8 of each of the wave's pieces; rows behind the last are read from the last one
+    const int8_t* base[PPW];
+    uint32_t off[PPW];
     {
         const int pr = lane >> 3, pc = lane & 7;
 #pragma unroll
         for (int s = 0; s < PPW; ++s) {
             const int q = min(s * NW + wave, PIECES - 1);
-            const int R = q * 8 + pr;
-            if (R < BM) {
-                src[s] = g.A + min(row0 + R, g.rows - 1) * g.lda + (pc ^ (R & 7)) * 16;
+            if (q * 8 < BM) {
+                const int R = q * 8 + pr;
+                base[s] = g.A + row0 * g.lda;
+                off[s] = (uint32_t)(min((int64_t)R, g.rows - 1 - row0) * g.lda) + (pc ^ (R & 7)) * 16;
             } else {
-                const int b = R - BM, key = (b & 3) | (((b >> KB) & 1) << 2);
-                src[s] = g.B + min(col0 + b, g.N - 1) * g.ldb + (pc ^ key) * 16;
+                const int R = q * 8 - BM + pr, key = (R & 3) | (((R >> KB) & 1) << 2);
+                base[s] = g.B + col0 * g.ldb;
+                off[s] = (uint32_t)(min((int64_t)R, g.N - 1 - col0) * g.ldb) + (pc ^ key) * 16;
             }
-            dst[s] = q * 1024;
         }
     }
-    auto issue = [&](int kt, int buf) {
+    const int first = slice * g.steps_per_split, steps = min(g.steps_per_split, g.steps - first);
+    auto request = [&](int kt, int stage) {              // (behind the last step: the last one again, which nothing reads)
+        const int64_t k = (int64_t)(first + min(kt, steps - 1)) * 128;
 #pragma unroll
         for (int s = 0; s < PPW; ++s)
-            __builtin_amdgcn_global_load_lds((glb_ptr_t)(src[s] + (int64_t)kt * 128), (lds_ptr_t)(lds + buf * STAGE_BYTES + dst[s]), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((glb_ptr_t)(base[s] + k + off[s]), (lds_ptr_t)(lds + stage * STAGE_BYTES + min(s * NW + wave, PIECES - 1) * 1024), 16, 0, 0);
     };
-    issue(0, 0);
+#pragma unroll
+    for (int st = 0; st < STAGES; ++st) request(st, st);
     const int x0 = (fq ^ (fr & 7)) * 16;
-    const int a_off = (wr * 16 * FM + fr) * 128;
-    const int b_off = (BM + wc * 16 * FN + (fr >> 2) * 4 * FN + (fr & 3)) * 128;
-    for (int kt = 0; kt < g.steps; ++kt) {
-        const int buf = kt & 1;
-        wait_vmcnt<0>();
+    const int a_off = (wr * 16 * FM + fr) * 128 + x0;
+    const int b_off = (BM + wc * 16 * FN + (fr >> 2) * RUN + (fr & 3)) * 128 + x0;
+    i32x4 af[2][FM], bf[2][FN];
+    auto read = [&](int half, int stage) {
+        const char* a = lds + ((stage * STAGE_BYTES + a_off) ^ (half * 64));
+        const char* b = lds + ((stage * STAGE_BYTES + b_off) ^ (half * 64));
+#pragma unroll
+        for (int j = 0; j < FN; ++j) bf[half][j] = *(const i32x4*)(b + j * 4 * 128);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) af[half][i] = *(const i32x4*)(a + i * 16 * 128);
+    };
+    auto multiply = [&](int half) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[half][j], af[half][i], acc[i][j], 0, 0, 0);
+    };
+    wait_vmcnt<(STAGES - 1) * PPW>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(0, 0);
+    int stage = 0;
+    for (int kt = 0; kt < steps; ++kt) {
+        const int next = stage + 1 == STAGES ? 0 : stage + 1;
+        __builtin_amdgcn_sched_barrier(0);
+        read(1, stage);
+        multiply(0);
+#pragma unroll
+        for (int s = 0; s < READS; ++s) {
+            __builtin_amdgcn_sched_group_barrier(0x008, PACE1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // this wave's reads of the stage are done and its requests of the next one have landed; behind the barrier so are everyone's
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        wait_vmcnt<(STAGES - 2) * PPW>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (kt + 1 < g.steps) issue(kt + 1, buf ^ 1);
-        const char* a_base = lds + buf * STAGE_BYTES + a_off;
-        const char* b_base = lds + buf * STAGE_BYTES + b_off;
+        __builtin_amdgcn_sched_barrier(0);
+        read(0, next);
+        request(kt + STAGES, stage);
+        multiply(1);
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            const int x = x0 ^ (ks * 64);
-            i32x4 af[FM], bf[FN];
-#pragma unroll
-            for (int j = 0; j < FN; ++j) bf[j] = *(const i32x4*)(b_base + j * 4 * 128 + x);
-#pragma unroll
-            for (int i = 0; i < FM; ++i) af[i] = *(const i32x4*)(a_base + i * 16 * 128 + x);
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[j], af[i], acc[i][j], 0, 0, 0);
+        for (int s = 0; s < READS; ++s) {
+            __builtin_amdgcn_sched_group_barrier(0x008, PACE2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
-    }
-
-    const int64_t n0 = col0 + wc * 16 * FN + fq * 4 * FN, left = g.N - n0;
-    if (left <= 0) return;
-    float sb[4 * FN], bias[4 * FN];
 #pragma unroll
-    for (int c = 0; c < 4 * FN; ++c) {
-        const int64_t n = min(n0 + c, g.N - 1);
-        sb[c] = g.sb ? g.sb[n] : 1.f;
-        bias[c] = g.bias ? load_as_f32(g.bias, n, g.dtype) : 0.f;
+        for (int s = 0; s < PPW; ++s) {
+            __builtin_amdgcn_sched_group_barrier(0x008, PACE2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        stage = next;
     }
+    wait_vmcnt<0>();                                     // (the requests behind the last step land before the LDS is given up)
+
+    const int64_t n0 = col0 + wc * 16 * FN + fq * RUN;
+    if (g.slab) {
+        int32_t* slab = g.slab + ((int64_t)slice * g.tiles_m * BM + row0 + wr * 16 * FM + fr) * ((int64_t)g.tiles_n * BN) + n0;
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) *(i32x4*)(slab + (int64_t)i * 16 * g.tiles_n * BN + 4 * j) = acc[i][j];
+        return;
+    }
+    const int64_t left = g.N - n0;
+    if (left <= 0) return;
+    // everything the epilogue reads is requested at once (loaded row by row it costs a trip to memory per row: 4 us of a 256 x 256 tile)
     const int64_t group0 = (row0 / 16 + wr * FM) / PLANES;
+    float sa[FM / PLANES], sb[RUN], bias[RUN];
+#pragma unroll
+    for (int i = 0; i < FM / PLANES; ++i) sa[i] = g.sa[min((group0 + i) * 16 + fr, g.M - 1)];
+#pragma unroll
+    for (int c = 0; c < RUN; ++c) sb[c] = 1.f, bias[c] = 0.f;
+    if (g.sb) load_run<RUN>(g.sb + n0, left, sb);
+    if (g.bias) {
+        if (g.dtype == SLIM_DTYPE_F32) load_run<RUN>((const float*)g.bias + n0, left, bias);
+        else if (g.dtype == SLIM_DTYPE_BF16) load_run<RUN>((const bf16_t*)g.bias + n0, left, bias);
+        else load_run<RUN>((const _Float16*)g.bias + n0, left, bias);
+    }
 #pragma unroll
     for (int i = 0; i < FM / PLANES; ++i) {
         const int64_t m = (group0 + i) * 16 + fr;
         if (m >= g.M) continue;
-        const float sa = g.sa[m];
         auto value = [&](int c) {
-            float v = (float)acc[i * PLANES][c >> 2][c & 3];
+            int sums[PLANES];
 #pragma unroll
-            for (int p = 1; p < PLANES; ++p) v = v * 256.f + (float)acc[i * PLANES + p][c >> 2][c & 3];
-            v = (v * sa) * sb[c];
+            for (int p = 0; p < PLANES; ++p) sums[p] = acc[i * PLANES + p][c >> 2][c & 3];
+            const float v = (join_planes<PLANES>(sums, 1) * sa[i]) * sb[c];
             return g.bias ? v + bias[c] : v;
         };
-        if (g.dtype == SLIM_DTYPE_F32) store_row<4 * FN>((float*)g.out + m * g.ldo + n0, left, value);
-        else if (g.dtype == SLIM_DTYPE_BF16) store_row<4 * FN>((bf16_t*)g.out + m * g.ldo + n0, left, [&](int c) { return f32_to_bf16(value(c)); });
-        else store_row<4 * FN>((_Float16*)g.out + m * g.ldo + n0, left, [&](int c) { return (_Float16)value(c); });
+        if (g.dtype == SLIM_DTYPE_F32) store_row<RUN>((float*)g.out + m * g.ldo + n0, left, value);
+        else if (g.dtype == SLIM_DTYPE_BF16) store_row<RUN>((bf16_t*)g.out + m * g.ldo + n0, left, [&](int c) { return f32_to_bf16(value(c)); });
+        else store_row<RUN>((_Float16*)g.out + m * g.ldo + n0, left, [&](int c) { return (_Float16)value(c); });
     }
 }
 
-template <int PLANES, int FM, int FN, int WM, int WN>
-int launch_gemm8(Gemm8Args g, hipStream_t st) {
-    constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN, bytes = 2 * (BM + BN) * 128;
-    g.tiles_m = (int)ceil_div64(g.rows, BM);
-    g.tiles_n = (int)ceil_div64(g.N, BN);
-    auto kernel = gemm8_kernel<PLANES, FM, FN, WM, WN>;
-    SLIM_REQUIRE((int64_t)g.tiles_m * g.tiles_n * 64 * WM * WN < (int64_t)1 << 32, "gemm8: the result is too large for one launch");
+// The slices' sums added (whole numbers: any order gives the same), planes joined, scaled and rounded: a thread per four columns.
+template <int PLANES>
+__global__ __launch_bounds__(256) void join_slices_kernel(const Gemm8Args g, int64_t slab_rows, int64_t slab_cols) {
+    const int64_t quads = (g.N + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t m = i / quads, n = (i - m * quads) * 4;
+    if (m >= g.M) return;
+    i32x4 sum[PLANES];
+#pragma unroll
+    for (int p = 0; p < PLANES; ++p) sum[p] = i32x4{0, 0, 0, 0};
+    const int32_t* src = g.slab + ((m / 16) * 16 * PLANES + m % 16) * slab_cols + n;
+    for (int z = 0; z < g.splits; ++z, src += slab_rows * slab_cols)
+#pragma unroll
+        for (int p = 0; p < PLANES; ++p) sum[p] += *(const i32x4*)(src + p * 16 * slab_cols);
+    const float sa = g.sa[m];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        if (n + c >= g.N) break;
+        int sums[PLANES];
+#pragma unroll
+        for (int p = 0; p < PLANES; ++p) sums[p] = sum[p][c];
+        float v = (join_planes<PLANES>(sums, 1) * sa) * (g.sb ? g.sb[n + c] : 1.f);
+        if (g.bias) v += load_as_f32(g.bias, n + c, g.dtype);
+        store_as(g.out, m * g.ldo + n + c, g.dtype, v);
+    }
+}
+
+// ---- which tile, how many slices ------------------------------------------------------------------------------------
+// Every tile's time, as measured over 32 to 4096 rows of weights 1024 x 1024 to 5120 x 13824 (us): a workgroup's start and end, a
+// 128-byte step while it has its CU to itself (few workgroups) and while all CUs, and both places of a CU where there are two, are
+// taken.  Larger tiles need fewer bytes per product (256 x 256: 2.3e15 operations/s at 4096 x 11008 x 4096, 128 x 128: 1.7e15),
+// smaller ones fill the chip sooner (300 x 4096 x 4096: 64 x 128 12 us, 256 x 256 38 us).  Slices of the reduction pay where tiles
+// alone leave CUs idle over a long reduction (64 x 5120 x 13824: four slices 19 us, one 31 us), for the pass that adds them.
+struct Tile {
+    int bm, bn, places;                                  // workgroups that share a CU
+    double ends, alone, full;
+};
+template <int PLANES>
+struct Tiles {
+    static constexpr int count = 4;
+    static constexpr Tile list[4] = {{256, 256, 1, 7.0, 1.02, 1.60}, {128, 256, 1, 5.0, 0.60, 0.97}, {128, 128, 1, 4.3, 0.40, 0.55}, {64, 128, 2, 3.5, 0.28, 0.57}};
+};
+template <>
+struct Tiles<3> {                                        // (a wave's rows are a multiple of 48)
+    static constexpr int count = 2;
+    static constexpr Tile list[2] = {{192, 256, 1, 6.0, 0.80, 1.25}, {96, 128, 1, 4.0, 0.35, 0.50}};
+};
+struct Plan {
+    int tile = 0, splits = 1, steps_per_split = 0;
+    int64_t tiles_m = 0, tiles_n = 0, slab_rows = 0, slab_cols = 0;
+    int64_t slab_bytes() const { return splits > 1 ? splits * slab_rows * slab_cols * 4 : 0; }
+};
+template <int PLANES>
+Plan plan_gemm8(int64_t rows, int64_t N, int64_t steps) {
+    Plan best;
+    double best_time = 1e30;
+    for (int k = 0; k < Tiles<PLANES>::count; ++k) {
+        const Tile t = Tiles<PLANES>::list[k];
+        const int64_t tiles_m = ceil_div64(rows, t.bm), tiles_n = ceil_div64(N, t.bn), tiles = tiles_m * tiles_n;
+        for (int splits = 1; splits <= 8 && (splits == 1 || (steps >= 8 * splits && tiles * splits <= 256)); splits *= 2) {
+            const int64_t each = ceil_div64(steps, splits), groups = tiles * splits, slots = 256 * t.places;
+            const int64_t rest = groups % slots;
+            auto round = [&](int64_t n) {                // n workgroups, at most `slots`
+                const double busy = t.places == 2 ? (n > 256 ? 1.0 : 0.0) : n / 256.0;
+                return t.ends + each * (t.alone + (t.full - t.alone) * busy);
+            };
+            double time = (groups / slots) * round(slots) + (rest ? round(rest) : 0.0);
+            if (splits > 1) time += 3.0 + 2.0 * splits * tiles * t.bm * t.bn * 4 / 4e6;
+            if (time < best_time) {
+                best_time = time;
+                best.tile = k, best.splits = (int)ceil_div64(steps, each), best.steps_per_split = (int)each;
+                best.tiles_m = tiles_m, best.tiles_n = tiles_n, best.slab_rows = tiles_m * t.bm, best.slab_cols = tiles_n * t.bn;
+            }
+        }
+    }
+    return best;
+}
+
+template <int PLANES, int TILE, int FM, int FN, int WM, int WN, int STAGES, int OCC>
+int launch_gemm8(const Gemm8Args& g, const Plan& p, hipStream_t st) {
+    constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN, bytes = STAGES * (BM + BN) * 128;
+    const int64_t blocks = p.tiles_m * p.tiles_n * p.splits;
+    static_assert(Tiles<PLANES>::list[TILE].bm == BM && Tiles<PLANES>::list[TILE].bn == BN, "the plan's tile");
+    SLIM_REQUIRE(blocks * 64 * WM * WN < (int64_t)1 << 32 && blocks < 0x7fffffff, "gemm8: the result is too large for one launch");
+    auto kernel = gemm8_kernel<PLANES, FM, FN, WM, WN, STAGES, OCC>;
     SLIM_HIP(slim_allow_dynamic_lds((const void*)kernel, bytes));
-    kernel<<<(unsigned)((int64_t)g.tiles_m * g.tiles_n), 64 * WM * WN, bytes, st>>>(g);
+    kernel<<<(unsigned)blocks, 64 * WM * WN, bytes, st>>>(g);
     SLIM_LAUNCH_CHECK();
     return SLIM_OK;
 }
 
 template <int PLANES>
-int gemm8(const Gemm8Args& g, hipStream_t st) {
-    SLIM_PROF("gemm8", st, (double)g.rows * g.steps * 128 + (double)g.N * g.steps * 128 + (double)g.M * g.N * 2,
+int gemm8(Gemm8Args g, void* slab, hipStream_t st) {
+    SLIM_PROF("gemm8", st, (double)g.rows * g.steps * 128 + (double)g.N * g.steps * 128 + (double)g.M * g.N * (g.dtype == SLIM_DTYPE_F32 ? 4 : 2),
               2.0 * g.rows * g.N * g.steps * 128);
-    return launch_gemm8<PLANES, PLANES == 3 ? 3 : 4, 4, 2, 2>(g, st);
+    const Plan p = plan_gemm8<PLANES>(g.rows, g.N, g.steps);
+    g.tiles_m = (int)p.tiles_m, g.tiles_n = (int)p.tiles_n;
+    g.splits = p.splits, g.steps_per_split = p.steps_per_split;
+    g.slab = p.splits > 1 ? (int32_t*)slab : nullptr;
+    int rc;
+    if constexpr (PLANES == 3) {
+        rc = p.tile == 0 ? launch_gemm8<3, 0, 6, 4, 2, 4, 2, 2>(g, p, st) : launch_gemm8<3, 1, 3, 2, 2, 4, 4, 2>(g, p, st);
+    } else {
+        if (p.tile == 0) rc = launch_gemm8<PLANES, 0, 8, 4, 2, 4, 2, 2>(g, p, st);
+        else if (p.tile == 1) rc = launch_gemm8<PLANES, 1, 4, 4, 2, 4, 3, 2>(g, p, st);
+        else if (p.tile == 2) rc = launch_gemm8<PLANES, 2, 4, 2, 2, 4, 4, 2>(g, p, st);
+        else rc = launch_gemm8<PLANES, 3, 2, 2, 2, 4, 3, 4>(g, p, st);
+    }
+    if (rc || p.splits == 1) return rc;
+    const int64_t threads = g.M * ((g.N + 3) / 4);
+    join_slices_kernel<PLANES><<<(unsigned)ceil_div64(threads, 256), 256, 0, st>>>(g, p.slab_rows, p.slab_cols);
+    SLIM_LAUNCH_CHECK();
+    return SLIM_OK;
+}
+
+// ---- few tokens -----------------------------------------------------------------------------------------------------
+// Up to 16 FM tokens: a workgroup owns 16 FN output channels over the whole reduction, each of its waves every NW-th 128-byte unit of
+// it, so nothing is joined outside the workgroup.  A wave keeps STAGES units of its own (the weight's rows and the tokens') under way
+// by LDS-DMA, eight whole 128-byte lines per request; as no other wave touches them it waits for its own requests only, and the one
+// barrier is that in front of the sums' addition.  (Loaded straight into the matrix instructions' layout, 16 rows by 64 bytes a
+// request, the weight takes half as long again.)
+struct RingArgs {
+    const int8_t* A;                                     // codes of the tokens
+    int64_t lda;
+    const float* sa;
+    const int8_t* B;
+    int64_t ldb;
+    const float* sb;
+    const void* bias;
+    void* out;
+    int64_t ldo;
+    int dtype, M, N, units;
+};
+template <int FM, int FN, int NW, int STAGES>
+__global__ __launch_bounds__(64 * NW) void ring8_kernel(const RingArgs g) {
+    constexpr int REQ = 2 * FM + 2 * FN, UNIT = REQ * 1024;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * 16 * FN;
+    char* const ring = lds + wave * STAGES * UNIT;
+    uint32_t off[REQ];                                   // a request: eight rows, lane / 8, of which it takes piece (lane % 8) ^ row
+    {
+        const int pr = lane >> 3, pc = (lane & 7) ^ pr;
+#pragma unroll
+        for (int s = 0; s < REQ; ++s)
+            off[s] = (s < 2 * FM ? (uint32_t)(min(s * 8 + pr, g.M - 1) * g.lda) : (uint32_t)(min((int64_t)(s - 2 * FM) * 8 + pr, g.N - 1 - n0) * g.ldb)) + pc * 16;
+    }
+    const int8_t* const b0 = g.B + n0 * g.ldb;
+    const int mine = wave < g.units ? (g.units - wave + NW - 1) / NW : 0;
+    auto request = [&](int i, int stage) {
+        const int64_t k = (int64_t)(wave + i * NW) * 128;
+#pragma unroll
+        for (int s = 0; s < REQ; ++s)
+            __builtin_amdgcn_global_load_lds((glb_ptr_t)((s < 2 * FM ? g.A : b0) + k + off[s]), (lds_ptr_t)(ring + stage * UNIT + s * 1024), 16, 0, 0);
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i)
+        if (i < mine) request(i, i);
+    i32x4 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+    const int x0 = fr * 128 + (fq ^ (fr & 7)) * 16;
+    int stage = 0;
+    for (int i = 0; i < mine; ++i) {
+        // the oldest unit has landed once only the younger ones are outstanding (at the end there are fewer of them: wait for all)
+        if (i + STAGES <= mine) wait_vmcnt<(STAGES - 1) * REQ>();
+        else wait_vmcnt<0>();
+        const char* unit = ring + stage * UNIT;
+        i32x4 a[FM][2], b[FN][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int j = 0; j < FM; ++j) a[j][h] = *(const i32x4*)(unit + j * 2048 + (x0 ^ (h * 64)));
+#pragma unroll
+            for (int j = 0; j < FN; ++j) b[j][h] = *(const i32x4*)(unit + (FM + j) * 2048 + (x0 ^ (h * 64)));
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");               // (read before it is requested again)
+        if (i + STAGES < mine) request(i + STAGES, stage);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int f = 0; f < FM; ++f) acc[f][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b[j][h], a[f][h], acc[f][j], 0, 0, 0);
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+    }
+    // every wave's sums over its own ring, nothing of which is under way any more
+    i32x4* const sums = (i32x4*)ring;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) sums[(i * FN + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    // a result per thread and turn: channel n of token m (the instruction's rows are channels, its columns tokens)
+    for (int t = threadIdx.x; t < 256 * FM * FN; t += 64 * NW) {
+        const int n = t % (16 * FN), m = t / (16 * FN);
+        if (m >= g.M || n0 + n >= g.N) continue;
+        const int at = ((m >> 4) * FN + (n >> 4)) * 64 + ((n & 15) >> 2) * 16 + (m & 15);
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) sum += ((const int*)(lds + w * STAGES * UNIT))[at * 4 + (n & 3)];
+        float v = ((float)sum * g.sa[m]) * g.sb[n0 + n];
+        if (g.bias) v += load_as_f32(g.bias, n0 + n, g.dtype);
+        store_as(g.out, m * g.ldo + n0 + n, g.dtype, v);
+    }
+}
+
+template <int FM, int FN, int NW, int STAGES>
+int launch_ring8_as(const RingArgs& g, hipStream_t st) {
+    constexpr int bytes = NW * STAGES * (FM + FN) * 2048;
+    auto kernel = ring8_kernel<FM, FN, NW, STAGES>;
+    SLIM_HIP(slim_allow_dynamic_lds((const void*)kernel, bytes));
+    kernel<<<(unsigned)ceil_div64(g.N, 16 * FN), 64 * NW, bytes, st>>>(g);
+    SLIM_LAUNCH_CHECK();
+    return SLIM_OK;
+}
+// Measured over both (us with the tokens' quantisation, weights 4096 x 4096, 11008 x 4096 and 5120 x 13824): sixteen channels and
+// eight waves 7.0, 13.8 and 21.5 for 16 tokens, 32 channels and four waves 8.0, 11.5 and 18.0; 8.2, 15.8 and 24.3 against 8.9, 13.5 and
+// 19.2 for 32.  From 33 tokens on and with many channels the tiles above share the tokens' codes better (64 x 11008 x 4096: 16.8
+// against 20.3, but 64 x 5120 x 13824: 27.2 against 24.4).
+bool takes_ring(int64_t M, int64_t N) { return M <= 32 || (M <= 64 && N <= 8192); }
+int launch_ring8(const RingArgs& g, hipStream_t st) {
+    const bool narrow = g.N <= 4096;
+    if (g.M <= 16) return narrow ? launch_ring8_as<1, 1, 8, 3>(g, st) : launch_ring8_as<1, 2, 4, 3>(g, st);
+    if (g.M <= 32) return narrow ? launch_ring8_as<2, 1, 8, 2>(g, st) : launch_ring8_as<2, 2, 4, 2>(g, st);
+    return narrow ? launch_ring8_as<4, 1, 8, 2>(g, st) : launch_ring8_as<4, 2, 4, 2>(g, st);
+}
+
+// ---- one or two tokens ----------------------------------------------------------------------------------------------
+// A product with one or two tokens reads the weight once and computes next to nothing, so it goes through the dot instructions and
+// the loads are laid out for memory alone: a wave's load is 1024 consecutive bytes of one row (in the matrix instructions' layout, 16
+// rows by 64 bytes, the same bytes take 1.5 times as long: 5120 x 13824, one token: 14.7 us against 21.4).  The workgroup quantises
+// the tokens itself (NP pieces of eight channels per thread, as in quantize_rows_kernel) and keeps them in LDS, so one launch does
+// it all; the tokens are requested before the weight, as loads return in order, and quantised while it travels.  A wave walks groups of
+// R rows with U loads of each under way, across the groups' ends.
+struct TokenArgs {
+    const void* x;
+    int64_t ldx;
+    const int8_t* B;
+    int64_t ldb;
+    const float* sb;
+    const void* bias;
+    void* out;
+    int64_t ldo;
+    int dtype, N, K;
+};
+template <typename T, int M, int NP, int R>
+__global__ __launch_bounds__(512) void token8_kernel(const TokenArgs g) {
+    constexpr int U = 4;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int waves = blockDim.x >> 6, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row_bytes = (g.K + 127) / 128 * 128, chunks = (row_bytes + 1023) / 1024, ldl = chunks * 1024;
+    uint32_t* const part = (uint32_t*)lds;               // [waves][M]
+    char* const codes = lds + 64;
+    float keep[M][NP][8];
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int c = (i * (int)blockDim.x + (int)threadIdx.x) * 8;
+            load8((const T*)g.x + m * g.ldx + c, (int64_t)g.K - c, keep[m][i]);
+        }
+    // step s of this wave: chunk s % chunks of its group s / chunks; group v holds the rows (v * all waves + this wave) * R ...
+    const int all = gridDim.x * waves, me = blockIdx.x * waves + wave, groups = (g.N + R - 1) / R, mine = me < groups ? (groups - me + all - 1) / all : 0;
+    const int steps = mine * chunks;
+    i32x4 buf[U][R];
+    int load_chunk = 0;
+    int64_t load_row = (int64_t)me * R;
+    auto load = [&](int i) {
+        const int o = min(load_chunk * 1024 + lane * 16, row_bytes - 16);
+#pragma unroll
+        for (int r = 0; r < R; ++r) buf[i][r] = *(const i32x4*)(g.B + min(load_row + r, (int64_t)g.N - 1) * g.ldb + o);
+        if (++load_chunk == chunks) load_chunk = 0, load_row += (int64_t)all * R;
+    };
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+        if (i < steps) load(i);
+    float scale[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t b = f32_bits(keep[m][i][j]) & 0x7fffffffu;
+                top = b > top ? b : top;
+            }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const uint32_t b = (uint32_t)__shfl_xor((int)top, o, 64);
+            top = b > top ? b : top;
+        }
+        if (lane == 0) part[wave * M + m] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        uint32_t top = 0;
+        for (int i = 0; i < waves; ++i) top = max(top, part[i * M + m]);
+        const RowScale s = row_scale<1>(top);
+        scale[m] = s.scale;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int c = (i * (int)blockDim.x + (int)threadIdx.x) * 8;
+            if (c >= ldl) continue;
+            if (s.none) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) keep[m][i][j] = 0.f;
+            }
+            store_codes<1>(keep[m][i], s.inverse, (int8_t*)codes, ldl, m, c);
+        }
+    }
+    __syncthreads();
+    int acc[R][M];
+    auto clear = [&]() {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int m = 0; m < M; ++m) acc[r][m] = 0;
+    };
+    clear();
+    int chunk = 0;
+    int64_t row = (int64_t)me * R;
+    for (int s = 0; s < steps; s += U) {
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            if (s + i >= steps) break;
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                const i32x4 x = *(const i32x4*)(codes + m * ldl + chunk * 1024 + lane * 16);
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[r][m] = __builtin_amdgcn_sdot4(buf[i][r][j], x[j], acc[r][m], false);
+            }
+            if (s + i + U < steps) load(i);
+            if (++chunk < chunks) continue;
+            chunk = 0;
+            int sum = 0;
+            float sx = scale[0];
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int m = 0; m < M; ++m) {
+#pragma unroll
+                    for (int o = 32; o > 0; o >>= 1) acc[r][m] += __shfl_xor(acc[r][m], o, 64);
+                    if (lane == r * M + m) sum = acc[r][m], sx = scale[m];
+                }
+            const int m = lane % M;
+            const int64_t n = row + lane / M;
+            if (lane < R * M && n < g.N) {               // lane r * M + m writes row r's result for token m
+                float v = ((float)sum * sx) * g.sb[n];
+                if (g.bias) v += load_as_f32(g.bias, n, g.dtype);
+                store_as(g.out, m * g.ldo + n, g.dtype, v);
+            }
+            row += (int64_t)all * R;
+            clear();
+        }
+    }
+}
+template <typename T, int M, int NP>
+int launch_token8(const TokenArgs& g, int waves, hipStream_t st) {
+    const int bytes = 64 + M * (int)(ceil_div64(pad128(g.K), 1024) * 1024);
+    // (two rows a wave and up to 768 workgroups, four rows and 512: 6.5 and 6.6 us at 4096 x 4096, 12.0 and 10.0 at 11008 x 4096)
+    const int64_t pairs = ceil_div64(g.N, waves * 2), fours = ceil_div64(g.N, waves * 4);
+    if (g.N < 8192) token8_kernel<T, M, NP, 2><<<(unsigned)(pairs < 768 ? pairs : 768), 64 * waves, bytes, st>>>(g);
+    else token8_kernel<T, M, NP, 4><<<(unsigned)(fours < 512 ? fours : 512), 64 * waves, bytes, st>>>(g);
+    SLIM_LAUNCH_CHECK();
+    return SLIM_OK;
+}
+
+// tokens kept in registers while they are quantised: NP pieces of eight channels per thread, 256 or 512 threads
+constexpr int TOKEN_PIECES[3] = {0, 7, 4};
+int token_waves(int64_t M, int64_t K) {                  // 0: not this kernel's
+    if (M > 2) return 0;
+    const int64_t pieces = ceil_div64(pad128(K), 1024) * 128;
+    return pieces <= TOKEN_PIECES[M] * 256 ? 4 : pieces <= TOKEN_PIECES[M] * 512 ? 8 : 0;
+}
+template <typename T>
+int token8(const TokenArgs& g, int64_t M, int waves, hipStream_t st) {
+    return M == 1 ? launch_token8<T, 1, TOKEN_PIECES[1]>(g, waves, st) : launch_token8<T, 2, TOKEN_PIECES[2]>(g, waves, st);
 }
 
 // ---- codes [N, K] -> codes [K, N] -----------------------------------------------------------------------------------
@@ -361,11 +838,6 @@ __global__ __launch_bounds__(256) void transpose8_kernel(const int8_t* __restric
         if (k0 + r < K && n0 + c < ldt) out[(k0 + r) * ldt + n0 + c] = tile[c][r];
 }
 
-int64_t pad128(int64_t k) { return (k + 127) / 128 * 128; }
-int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
-int planes_of(int dtype) { return dtype == SLIM_DTYPE_F32 ? 3 : 2; }
-bool known(int dtype) { return dtype == SLIM_DTYPE_F32 || dtype == SLIM_DTYPE_BF16 || dtype == SLIM_DTYPE_F16; }
-int64_t element_size(int dtype) { return dtype == SLIM_DTYPE_F32 ? 4 : 2; }
 
 }  // namespace
 
@@ -396,7 +868,9 @@ extern "C" int slim_transpose8(const int8_t* codes, int64_t N, int64_t K, int64_
     return SLIM_OK;
 }
 
-extern "C" int64_t slim_gemm8_workspace_bytes(int64_t M, int64_t N, int64_t K) { return 0; }
+extern "C" int64_t slim_gemm8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    return M > 0 && N > 0 && K > 0 && !takes_ring(M, N) ? plan_gemm8<1>(M, N, pad128(K) / 128).slab_bytes() : 0;
+}
 
 extern "C" int slim_gemm8_nt(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, const float* sb, int64_t M, int64_t N,
                              int64_t K, const void* bias, int dtype, void* out, int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -407,30 +881,42 @@ extern "C" int slim_gemm8_nt(const int8_t* a, int64_t lda, const float* sa, cons
                  "slim_gemm8_nt: rows of codes hold slim_rows8_ld(K) bytes and start at multiples of 16");
     SLIM_REQUIRE(workspace_bytes >= slim_gemm8_workspace_bytes(M, N, K) && (workspace || workspace_bytes == 0) && (uintptr_t)workspace % 16 == 0,
                  "slim_gemm8_nt: workspace too small or misaligned");
-    Gemm8Args g{a, b, lda, ldb, M, M, N, (int)(pad128(K) / 128), sa, sb, bias, out, ldo, dtype, 0, 0};
-    return gemm8<1>(g, (hipStream_t)stream);
+    SLIM_REQUIRE(lda < 1 << 23 && ldb < 1 << 23, "slim_gemm8_nt: rows of codes lie too far apart");
+    if (takes_ring(M, N)) return launch_ring8(RingArgs{a, lda, sa, b, ldb, sb, bias, out, ldo, dtype, (int)M, (int)N, (int)(pad128(K) / 128)}, (hipStream_t)stream);
+    Gemm8Args g{a, b, lda, ldb, M, M, N, (int)(pad128(K) / 128), sa, sb, bias, out, ldo, dtype, 0, 0, 1, 0, nullptr};
+    return gemm8<1>(g, workspace, (hipStream_t)stream);
 }
 
 extern "C" int64_t slim_linear8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    (void)N;
-    return M > 0 && K > 0 ? align256(M * pad128(K)) + align256(M * 4) : 0;
+    if (M <= 0 || N <= 0 || K <= 0 || token_waves(M, K)) return 0;
+    return align256(M * pad128(K)) + align256(M * 4) + slim_gemm8_workspace_bytes(M, N, K);
 }
 
 extern "C" int slim_linear8_forward(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, const int8_t* codes, const float* scale, int64_t N,
                                     const void* bias, void* y, int64_t ldy, void* workspace, int64_t workspace_bytes, void* stream) {
-    SLIM_REQUIRE(x && codes && scale && y && workspace && M > 0 && N > 0 && K > 0 && ldx >= K && ldy >= N, "slim_linear8_forward: bad arguments");
-    SLIM_REQUIRE(workspace_bytes >= slim_linear8_workspace_bytes(M, N, K) && (uintptr_t)workspace % 16 == 0,
-                 "slim_linear8_forward: workspace too small or misaligned");
+    SLIM_REQUIRE(x && codes && scale && y && M > 0 && N > 0 && K > 0 && ldx >= K && ldy >= N, "slim_linear8_forward: bad arguments");
+    const int64_t need = slim_linear8_workspace_bytes(M, N, K);
+    SLIM_REQUIRE(workspace_bytes >= need && (workspace || !need) && (uintptr_t)workspace % 16 == 0, "slim_linear8_forward: workspace too small or misaligned");
+    if (const int waves = token_waves(M, K)) {
+        SLIM_REQUIRE(known(dtype), "slim_linear8_forward: unknown element type %d", dtype);
+        SLIM_REQUIRE(N <= SLIM_INT8_MAX_DIM && (uintptr_t)codes % 16 == 0, "slim_linear8_forward: weight too large or misaligned");
+        const TokenArgs g{x, ldx, codes, pad128(K), scale, bias, y, ldy, dtype, (int)N, (int)K};
+        if (dtype == SLIM_DTYPE_F32) return token8<float>(g, M, waves, (hipStream_t)stream);
+        if (dtype == SLIM_DTYPE_BF16) return token8<bf16_t>(g, M, waves, (hipStream_t)stream);
+        return token8<_Float16>(g, M, waves, (hipStream_t)stream);
+    }
     int8_t* xc = (int8_t*)workspace;
     float* sx = (float*)(xc + align256(M * pad128(K)));
     const int rc = slim_quantize_rows8(x, dtype, M, K, ldx, xc, pad128(K), sx, stream);
     if (rc) return rc;
-    return slim_gemm8_nt(xc, pad128(K), sx, codes, pad128(K), scale, M, N, K, bias, dtype, y, ldy, nullptr, 0, stream);
+    char* slab = (char*)sx + align256(M * 4);
+    return slim_gemm8_nt(xc, pad128(K), sx, codes, pad128(K), scale, M, N, K, bias, dtype, y, ldy, slab, (char*)workspace + workspace_bytes - slab, stream);
 }
 
 extern "C" int64_t slim_linear8_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
-    (void)K;
-    return M > 0 && N > 0 && known(dtype) ? align256((M + 15) / 16 * 16 * planes_of(dtype) * pad128(N)) + align256(M * 4) : 0;
+    if (M <= 0 || N <= 0 || K <= 0 || !known(dtype)) return 0;
+    const int64_t rows = (M + 15) / 16 * 16 * planes_of(dtype);
+    return align256(rows * pad128(N)) + align256(M * 4) + (planes_of(dtype) == 3 ? plan_gemm8<3>(rows, K, pad128(N) / 128) : plan_gemm8<2>(rows, K, pad128(N) / 128)).slab_bytes();
 }
 
 extern "C" int slim_linear8_backward(const void* dy, int dtype, int64_t lddy, int64_t M, int64_t N, const int8_t* codes_t, const float* scale, int64_t K,
@@ -449,6 +935,7 @@ extern "C" int slim_linear8_backward(const void* dy, int dtype, int64_t lddy, in
     const int rc = planes == 3 ? quantize_rows_any<3>(dy, dtype, M, N, lddy, scale, q, ld, sq, st)
                                : quantize_rows_any<2>(dy, dtype, M, N, lddy, scale, q, ld, sq, st);
     if (rc) return rc;
-    Gemm8Args g{q, codes_t, ld, ld, rows, M, K, (int)(ld / 128), sq, nullptr, nullptr, dx, lddx, dtype, 0, 0};
-    return planes == 3 ? gemm8<3>(g, st) : gemm8<2>(g, st);
+    void* slab = (char*)sq + align256(M * 4);
+    Gemm8Args g{q, codes_t, ld, ld, rows, M, K, (int)(ld / 128), sq, nullptr, nullptr, dx, lddx, dtype, 0, 0, 1, 0, nullptr};
+    return planes == 3 ? gemm8<3>(g, slab, st) : gemm8<2>(g, slab, st);
 }

@@ -4,6 +4,9 @@ PyTorch is used for device memory and streams only: every function allocates its
 with torch, passes raw device pointers and the current HIP stream to libslim_hip.so, and
 returns torch tensors.  Inputs must live on a ROCm device; nothing here computes on the CPU.
 """
+import array
+import itertools
+import operator
 import os
 
 import torch
@@ -1078,58 +1081,81 @@ def linear24_forward_q4(x, vals, meta, sf, N, bias, qL, qR, r, qblock, a_div, ws
 
 # ---- linears in 8-bit integers ------------------------------------------------------------------------------
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-def _call_at(device, name, *args):
-    """_lib.call with `device` current and its current stream as the last argument."""
-    if device.index == torch.cuda.current_device():
-        _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
-        return
-    with torch.cuda.device(device):
-        _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
-
-
-def _dtype_code(t, name):
-    code = _DTYPES.get(t.dtype)
-    if code is None:
-        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-    return code
+def _call_at(index, name, *args):
+    """_lib.call with GPU `index` current and its current stream as the last argument (a product with one token takes the GPU
+    7 us: what a call costs the host counts)."""
+    fn = getattr(_lib.load(), name)
+    if index == _current_device():
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.raise_status(name, rc)
 
 
 def _rows8(t, name):
-    """(2-d tensor with consecutive elements in its rows, element type code); rows may lie further apart than their length."""
+    """(2-d tensor with consecutive elements in its rows, rows, columns, elements from row to row, element type code, GPU)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if not t.is_cuda:
+    index = t.get_device()
+    if index < 0:
         raise RuntimeError(f"{name} must be on the GPU: slim_amd has no CPU path (got device {t.device})")
-    code = _dtype_code(t, name)
-    if t.dim() != 2 or t.shape[1] == 0:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if t.dim() != 2 or t.size(1) == 0:
         raise ValueError(f"{name} must be a matrix with at least one column, got {tuple(t.shape)}")
-    if t.shape[0] > 1 and (t.stride(1) != 1 or t.stride(0) < t.shape[1]) or t.shape[1] > 1 and t.stride(1) != 1:
+    rows, cols = t.shape
+    if t.is_contiguous():
+        return t, rows, cols, cols, code, index
+    if cols > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < cols:
         t = t.contiguous()
-    return t, code
+        return t, rows, cols, cols, code, index
+    return t, rows, cols, t.stride(0) if rows > 1 else cols, code, index
 
 
-def _stride0(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _operand(t, dtype, index, name):
+    """A contiguous tensor of the given type on the given GPU."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.get_device() != index:
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} must be on the GPU: slim_amd has no CPU path (got device {t.device})")
+        raise ValueError(f"all tensors must be on one device, got cuda:{index} and {t.device} ({name})")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _codes8(t, rows, name):
-    """A contiguous int8 matrix of codes with `rows` rows (any number when None)."""
-    t = _chk(t, torch.int8, name)
-    if t.dim() != 2 or t.shape[0] == 0 or t.shape[1] % 128 or t.shape[1] == 0 or (rows is not None and t.shape[0] != rows):
-        raise ValueError(f"{name} must be [{'rows' if rows is None else rows}, a multiple of 128], got {tuple(t.shape)}")
+def _codes8(t, index, name):
+    """A contiguous int8 matrix of codes and its shape."""
+    t = _operand(t, torch.int8, index, name)
+    if t.dim() != 2 or t.numel() == 0 or t.size(1) % 128:
+        raise ValueError(f"{name} must be [rows, a multiple of 128], got {tuple(t.shape)}")
+    return t, t.size(0), t.size(1)
+
+
+def _vector(t, n, dtype, index, name):
+    t = _operand(t, dtype, index, name)
+    if t.numel() != n:
+        raise ValueError(f"{name} must hold {n} values, got {tuple(t.shape)}")
     return t
-
-
-def _same_device(first, *rest):
-    for t in rest:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"all tensors must be on one device, got {first.device} and {t.device}")
 
 
 def _pad128(k):
     return -(-k // 128) * 128
+
+
+def _gpu_of(t, name):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be on the GPU: slim_amd has no CPU path (got device {t.device})")
+    return t.get_device()
 
 
 def quantize_rows8(x):
@@ -1137,78 +1163,70 @@ def quantize_rows8(x):
     rint(x * (127 / a)) with a the row's largest magnitude, scale a / 127, zeros behind column K.  A row below 2^-100
     everywhere gets scale 0; one that holds an infinity or a NaN gets scale NaN.  Tokens of an activation, or output channels
     of a weight [N, K] (the operand of linear8_forward)."""
-    x, dt = _rows8(x, "x")
-    R, K = x.shape
-    codes = torch.empty(R, _pad128(K), dtype=torch.int8, device=x.device)
+    x, R, K, ld, dt, gpu = _rows8(x, "x")
+    codes = torch.empty((R, _pad128(K)), dtype=torch.int8, device=x.device)
     scale = torch.empty(R, dtype=torch.float32, device=x.device)
     if R:
-        _call_at(x.device, "slim_quantize_rows8", x.data_ptr(), dt, R, K, _stride0(x), codes.data_ptr(), codes.shape[1], scale.data_ptr())
+        _call_at(gpu, "slim_quantize_rows8", x.data_ptr(), dt, R, K, ld, codes.data_ptr(), _pad128(K), scale.data_ptr())
     return codes, scale
 
 
 def transpose8(codes, K):
     """Codes [K, N rounded up to 128] of the transposed matrix of codes [N, K rounded up to 128] (the operand of
     linear8_backward)."""
-    codes = _codes8(codes, None, "codes")
-    N = codes.shape[0]
-    if _pad128(K) != codes.shape[1]:
-        raise ValueError(f"codes of {K} columns have {_pad128(K)}, got {codes.shape[1]}")
-    out = torch.empty(K, _pad128(N), dtype=torch.int8, device=codes.device)
-    _call_at(codes.device, "slim_transpose8", codes.data_ptr(), N, K, codes.shape[1], out.data_ptr(), out.shape[1])
+    gpu = _gpu_of(codes, "codes")
+    codes, N, Kp = _codes8(codes, gpu, "codes")
+    if _pad128(K) != Kp:
+        raise ValueError(f"codes of {K} columns have {_pad128(K)}, got {Kp}")
+    out = torch.empty((K, _pad128(N)), dtype=torch.int8, device=codes.device)
+    _call_at(gpu, "slim_transpose8", codes.data_ptr(), N, K, Kp, out.data_ptr(), _pad128(N))
     return out
 
 
-def _vector(t, n, dtype, name):
-    t = _chk(t, dtype, name)
-    if t.numel() != n:
-        raise ValueError(f"{name} must hold {n} values, got {tuple(t.shape)}")
-    return t
+def _workspace(nbytes, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 def gemm8_nt(a, sa, b, sb, bias=None, out_dtype=BF16, K=None):
     """out [M, N] = (a @ b.T) * sa[:, None] * sb (+ bias) for codes a [M, Kp], b [N, Kp] with scales sa [M], sb [N] as
     quantize_rows8 makes them: the sum in whole numbers, the rest in fp32, rounded once to out_dtype.  K: the number of columns
     that are not padding (all when None), at most 131071."""
-    a, b = _codes8(a, None, "a"), _codes8(b, None, "b")
-    M, Kp = a.shape
-    N = b.shape[0]
-    if b.shape[1] != Kp:
-        raise ValueError(f"a and b must have equally long rows, got {Kp} and {b.shape[1]}")
+    gpu = _gpu_of(a, "a")
+    a, M, Kp = _codes8(a, gpu, "a")
+    b, N, Kb = _codes8(b, gpu, "b")
+    if Kb != Kp:
+        raise ValueError(f"a and b must have equally long rows, got {Kp} and {Kb}")
     if out_dtype not in _DTYPES:
         raise TypeError(f"out_dtype must be float32, bfloat16 or float16, got {out_dtype}")
     K = Kp if K is None else int(K)
     if not Kp - 128 < K <= Kp:
         raise ValueError(f"gemm8_nt: K must lie in ({Kp - 128}, {Kp}], got {K}")
-    sa, sb = _vector(sa, M, torch.float32, "sa"), _vector(sb, N, torch.float32, "sb")
+    sa, sb = _vector(sa, M, torch.float32, gpu, "sa"), _vector(sb, N, torch.float32, gpu, "sb")
     if bias is not None:
-        bias = _vector(bias, N, out_dtype, "bias")
-    _same_device(a, b, sa, sb, bias)
-    out = torch.empty(M, N, dtype=out_dtype, device=a.device)
-    nb = _lib.query("slim_gemm8_workspace_bytes", M, N, K)
-    ws = _ws(nb, a.device)
-    _call_at(a.device, "slim_gemm8_nt", a.data_ptr(), Kp, sa.data_ptr(), b.data_ptr(), Kp, sb.data_ptr(), M, N, K, _p(bias), _DTYPES[out_dtype],
-             out.data_ptr(), N, ws.data_ptr(), ws.numel())
+        bias = _vector(bias, N, out_dtype, gpu, "bias")
+    out = torch.empty((M, N), dtype=out_dtype, device=a.device)
+    need = _lib.query("slim_gemm8_workspace_bytes", M, N, K)
+    ws = _workspace(need, a.device)
+    _call_at(gpu, "slim_gemm8_nt", a.data_ptr(), Kp, sa.data_ptr(), b.data_ptr(), Kp, sb.data_ptr(), M, N, K, _p(bias), _DTYPES[out_dtype], out.data_ptr(), N,
+             _p(ws), need)
     return out
 
 
 def linear8_forward(x, codes, scale, bias=None):
     """y [M, N] = x [M, K], quantised token by token (quantize_rows8), times the weight kept as codes [N, Kp] and scale [N],
     plus bias [N]; y and bias have the type of x (fp32, bf16 or fp16)."""
-    x, dt = _rows8(x, "x")
-    M, K = x.shape
-    codes = _codes8(codes, None, "codes")
-    N = codes.shape[0]
-    if codes.shape[1] != _pad128(K):
-        raise ValueError(f"codes of a weight with {K} input channels have {_pad128(K)} columns, got {codes.shape[1]}")
-    scale = _vector(scale, N, torch.float32, "scale")
+    x, M, K, ld, dt, gpu = _rows8(x, "x")
+    codes, N, Kp = _codes8(codes, gpu, "codes")
+    if Kp != _pad128(K):
+        raise ValueError(f"codes of a weight with {K} input channels have {_pad128(K)} columns, got {Kp}")
+    scale = _vector(scale, N, torch.float32, gpu, "scale")
     if bias is not None:
-        bias = _vector(bias, N, x.dtype, "bias")
-    _same_device(x, codes, scale, bias)
-    y = torch.empty(M, N, dtype=x.dtype, device=x.device)
+        bias = _vector(bias, N, x.dtype, gpu, "bias")
+    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
     if M:
-        ws = _ws(_lib.query("slim_linear8_workspace_bytes", M, N, K), x.device)
-        _call_at(x.device, "slim_linear8_forward", x.data_ptr(), dt, _stride0(x), M, K, codes.data_ptr(), scale.data_ptr(), N, _p(bias), y.data_ptr(), N,
-                 ws.data_ptr(), ws.numel())
+        need = _lib.query("slim_linear8_workspace_bytes", M, N, K)
+        ws = _workspace(need, x.device)
+        _call_at(gpu, "slim_linear8_forward", x.data_ptr(), dt, ld, M, K, codes.data_ptr(), scale.data_ptr(), N, _p(bias), y.data_ptr(), N, _p(ws), need)
     return y
 
 
@@ -1216,19 +1234,16 @@ def linear8_backward(dy, codes_t, scale):
     """dx [M, K] = (dy [M, N] * scale) @ codes: the gradient of linear8_forward with respect to x, the quantisation of x passed
     straight through.  codes_t [K, Np] from transpose8; dx has the type of dy.  dy * scale is kept as integers of 16 bits per row
     (24 for fp32), so a row's error is below sqrt(N / 12) 2^-15 (2^-23) of its norm."""
-    dy, dt = _rows8(dy, "dy")
-    M, N = dy.shape
-    codes_t = _codes8(codes_t, None, "codes_t")
-    K = codes_t.shape[0]
-    if codes_t.shape[1] != _pad128(N):
-        raise ValueError(f"codes_t of a weight with {N} output channels has {_pad128(N)} columns, got {codes_t.shape[1]}")
-    scale = _vector(scale, N, torch.float32, "scale")
-    _same_device(dy, codes_t, scale)
-    dx = torch.empty(M, K, dtype=dy.dtype, device=dy.device)
+    dy, M, N, ld, dt, gpu = _rows8(dy, "dy")
+    codes_t, K, Np = _codes8(codes_t, gpu, "codes_t")
+    if Np != _pad128(N):
+        raise ValueError(f"codes_t of a weight with {N} output channels has {_pad128(N)} columns, got {Np}")
+    scale = _vector(scale, N, torch.float32, gpu, "scale")
+    dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
     if M:
-        ws = _ws(_lib.query("slim_linear8_backward_workspace_bytes", M, N, K, dt), dy.device)
-        _call_at(dy.device, "slim_linear8_backward", dy.data_ptr(), dt, _stride0(dy), M, N, codes_t.data_ptr(), scale.data_ptr(), K, dx.data_ptr(), K,
-                 ws.data_ptr(), ws.numel())
+        need = _lib.query("slim_linear8_backward_workspace_bytes", M, N, K, dt)
+        ws = _workspace(need, dy.device)
+        _call_at(gpu, "slim_linear8_backward", dy.data_ptr(), dt, ld, M, N, codes_t.data_ptr(), scale.data_ptr(), K, dx.data_ptr(), K, _p(ws), need)
     return dx
 
 
@@ -1236,44 +1251,72 @@ def linear8_backward(dy, codes_t, scale):
 ADAMW_BLOCK = 512         # elements of a tensor that share a pair of scales (8-bit moments)
 
 
-def _dense(t, name):
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} must be on the GPU: slim_amd has no CPU path (got device {t.device})")
-    if t.layout != torch.strided:
-        raise TypeError(f"{name} must be a dense tensor, got {t.layout}")
+def _alike(tensors, dtype, index, sizes, name):
+    """Contiguous tensors of one type on one GPU, of the given sizes (any when None)."""
+    cls = torch.Tensor
+    if not (all(isinstance(t, cls) for t in tensors) and set(map(cls.get_device, tensors)) == {index} and all(t.layout == torch.strided for t in tensors)):
+        for t in tensors:
+            if not isinstance(t, cls):
+                raise TypeError(f"{name} must be torch.Tensors")
+            if not t.is_cuda:
+                raise RuntimeError(f"{name} must be on the GPU: slim_amd has no CPU path (got device {t.device})")
+            if t.layout != torch.strided:
+                raise TypeError(f"{name} must be dense tensors, got {t.layout}")
+        raise ValueError(f"{name} must be on one device")
+    if {t.dtype for t in tensors} != {dtype}:
+        raise ValueError(f"{name} must be {dtype}, got {sorted({str(t.dtype) for t in tensors})}")
+    if not all(map(cls.is_contiguous, tensors)):
+        raise ValueError(f"{name} must be contiguous")
+    if sizes is not None and list(map(cls.numel, tensors)) != sizes:
+        raise ValueError(f"{name} must have the parameters' sizes")
 
 
-def _addresses(tensors):
-    import ctypes
-    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+_dtype_of = operator.attrgetter("dtype")
 
 
-def _sizes(tensors):
-    import ctypes
-    return (ctypes.c_int64 * len(tensors))(*[t.numel() for t in tensors])
+def _plain(groups, index):
+    """Whether every (tensors, type, sizes or None) holds contiguous tensors of its type and sizes on GPU `index` (a quick check: an
+    optimizer step may have thousands of tensors; _alike says what is wrong)."""
+    cls = torch.Tensor
+    tensors = [t for g in groups for t in g[0]]
+    try:
+        return (set(map(cls.get_device, tensors)) == {index} and all(map(cls.is_contiguous, tensors)) and
+                all(set(map(_dtype_of, ts)) == {dtype} and (sizes is None or list(map(cls.numel, ts)) == sizes) for ts, dtype, sizes in groups))
+    except (TypeError, RuntimeError, AttributeError):
+        return False
+
+
+def _words(values):
+    """A host array of 64-bit words and its address."""
+    a = array.array("q", values)
+    return a, a.buffer_info()[0]
 
 
 def grad_norm(grads):
     """sqrt of the sum of squares over all tensors of a list (one element type, one device): a 0-d fp32 tensor, squares and
     sums in 64 bits.  Empty tensors count nothing; an empty list is refused."""
-    import ctypes
     grads = list(grads)
     if not grads:
         raise ValueError("grad_norm needs at least one tensor")
-    for g in grads:
-        _dense(g, "grads")
-        if g.dtype != grads[0].dtype or g.device != grads[0].device:
-            raise ValueError("grads must have one element type and one device")
-    dt, dev = _dtype_code(grads[0], "grads"), grads[0].device
-    full = [g if g.is_contiguous() else g.contiguous() for g in grads if g.numel()]
-    if not full:
-        return torch.zeros((), dtype=torch.float32, device=dev)
+    gpu = _gpu_of(grads[0], "grads")
+    if not _plain([(grads, grads[0].dtype, None)], gpu):
+        grads = [g if not isinstance(g, torch.Tensor) or g.layout != torch.strided else g.contiguous() for g in grads]
+        _alike(grads, grads[0].dtype, gpu, None, "grads")
+    dt, dev = _DTYPES.get(grads[0].dtype), grads[0].device
+    if dt is None:
+        raise TypeError(f"grads must be float32, bfloat16 or float16, got {grads[0].dtype}")
+    sizes = list(map(torch.Tensor.numel, grads))
+    if 0 in sizes:
+        grads = [g for g, n in zip(grads, sizes) if n]
+        sizes = [n for n in sizes if n]
+        if not grads:
+            return torch.zeros((), dtype=torch.float32, device=dev)
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    ws = _ws(_lib.query("slim_grad_norm_workspace_bytes", len(full)), dev)
-    ptrs, sizes = _addresses(full), _sizes(full)
-    _call_at(dev, "slim_grad_norm", ctypes.addressof(ptrs), ctypes.addressof(sizes), len(full), dt, norm.data_ptr(), ws.data_ptr(), ws.numel())
+    need = _lib.query("slim_grad_norm_workspace_bytes", len(grads))
+    ws = _workspace(need, dev)
+    ptrs, ptrs_at = _words(map(torch.Tensor.data_ptr, grads))
+    counts, counts_at = _words(sizes)
+    _call_at(gpu, "slim_grad_norm", ptrs_at, counts_at, len(grads), dt, norm.data_ptr(), ws.data_ptr(), need)
     return norm
 
 
@@ -1287,48 +1330,51 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, beta1=0.9, bet
     of 16-bit parameters, which are then their roundings.  norm (0-d fp32 tensor, grad_norm) with max_norm: the gradients are
     multiplied by min(1, max_norm / (norm + 1e-6)) as they are read.  step counts from 1.  Empty tensors are left alone.  A captured call
     replays with the step, lr and seed that it was captured with."""
-    import ctypes
-    lists = [list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), None if scales is None else list(scales), None if masters is None else list(masters)]
-    params, grads, ms, vs, ss, ws = lists
+    params, grads, ms, vs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
+    ss, ws = None if scales is None else list(scales), None if masters is None else list(masters)
     count = len(params)
-    if any(x is not None and len(x) != count for x in lists):
+    if any(x is not None and len(x) != count for x in (grads, ms, vs, ss, ws)):
         raise ValueError("adamw_step: all lists must be equally long")
     if not count:
         return
-    dtype, dev = params[0].dtype, params[0].device
-    dt = _dtype_code(params[0], "params")
-    moments = (torch.float32, torch.float32) if ss is None else (torch.float8_e4m3fn, torch.float8_e5m2)
+    gpu = _gpu_of(params[0], "params")
+    dtype = params[0].dtype
+    _alike(params[:1], dtype, gpu, None, "adamw_step: params")
+    dt = _DTYPES.get(dtype)
+    if dt is None:
+        raise TypeError(f"params must be float32, bfloat16 or float16, got {dtype}")
     if ws is not None and dtype == torch.float32:
         raise ValueError("adamw_step: fp32 parameters need no master copies")
+    try:
+        sizes = list(map(torch.Tensor.numel, params))
+    except TypeError:
+        sizes = None                                     # (not tensors: the checks below say so)
+    groups = [(params, dtype, sizes), (grads, dtype, sizes), (ms, torch.float32 if ss is None else torch.float8_e4m3fn, sizes),
+              (vs, torch.float32 if ss is None else torch.float8_e5m2, sizes)]
+    names = ["params", "grads", "exp_avgs", "exp_avg_sqs"]
+    if ss is not None:
+        groups.append((ss, torch.float32, [2 * -(-n // ADAMW_BLOCK) for n in sizes or []]))
+        names.append(f"scales ([ceil(n / {ADAMW_BLOCK}), 2])")
+    if ws is not None:
+        groups.append((ws, torch.float32, sizes))
+        names.append("masters")
+    if not _plain(groups, gpu):
+        for (tensors, want, n), name in zip(groups, names):
+            _alike(tensors, want, gpu, n, "adamw_step: " + name)
     if (norm is None) != (max_norm is None):
         raise ValueError("adamw_step: norm and max_norm go together")
-    checks = [(params, dtype, "params"), (grads, dtype, "grads"), (ms, moments[0], "exp_avgs"), (vs, moments[1], "exp_avg_sqs")]
-    if ws is not None:
-        checks.append((ws, torch.float32, "masters"))
-    sizes = [p.numel() for p in params]
-    for tensors, want, name in checks:
-        for t, n in zip(tensors, sizes):
-            _dense(t, name)
-            if t.dtype != want or t.device != dev or t.numel() != n or not t.is_contiguous():
-                raise ValueError(f"adamw_step: {name} must be contiguous {want} tensors on {dev} of the parameters' sizes")
-    if ss is not None:
-        for s, n in zip(ss, sizes):
-            _dense(s, "scales")
-            if s.dtype != torch.float32 or s.device != dev or tuple(s.shape) != (-(-n // ADAMW_BLOCK), 2) or not s.is_contiguous():
-                raise ValueError(f"adamw_step: scales must be contiguous fp32 [ceil(n / {ADAMW_BLOCK}), 2] tensors on {dev}")
     if norm is not None:
-        _dense(norm, "norm")
-        if norm.dtype != torch.float32 or norm.numel() != 1 or norm.device != dev:
-            raise ValueError("adamw_step: norm must be one fp32 value on the parameters' device")
+        norm = _vector(norm, 1, torch.float32, gpu, "norm")
     if 0 in sizes:
         keep = [i for i, n in enumerate(sizes) if n]
         params, grads, ms, vs, ss, ws = (None if x is None else [x[i] for i in keep] for x in (params, grads, ms, vs, ss, ws))
+        sizes = [sizes[i] for i in keep]
         if not keep:
             return
-    arrays = [None if x is None else _addresses(x) for x in (params, grads, ms, vs, ss, ws)]
-    numel = _sizes(params)
-    _call_at(dev, "slim_adamw_step", *[None if x is None else ctypes.addressof(x) for x in arrays], ctypes.addressof(numel), len(params), dt,
-             int(first_index), int(step), float(lr), float(beta1), float(beta2), float(eps), float(weight_decay), _p(norm),
-             0.0 if max_norm is None else float(max_norm), int(seed) & 0xffffffff)
-    for p in params:
-        torch.autograd.graph.increment_version(p)
+    lists = [x for x in (params, grads, ms, vs, ss, ws) if x is not None]
+    words, at = _words(itertools.chain(*(map(torch.Tensor.data_ptr, x) for x in lists), sizes))       # one array after another
+    starts = iter(range(at, at + words.itemsize * len(words), words.itemsize * len(params)))
+    arrays = [None if x is None else next(starts) for x in (params, grads, ms, vs, ss, ws)] + [next(starts)]
+    _call_at(gpu, "slim_adamw_step", *arrays, len(params), dt, int(first_index), int(step), float(lr), float(beta1), float(beta2), float(eps),
+             float(weight_decay), _p(norm), 0.0 if max_norm is None else float(max_norm), int(seed) & 0xffffffff)
+    torch.autograd.graph.increment_version(params)

@@ -17,6 +17,7 @@ def test_sizes():
     assert [lib.slim_rows8_ld(k) for k in (1, 127, 128, 129, 4096, 0, -3)] == [128, 128, 128, 256, 4096, 0, 0]
     assert [lib.slim_adamw_blocks(n) for n in (1, 512, 513, 0)] == [1, 1, 2, 0]
     assert lib.slim_linear8_workspace_bytes(5, 64, 100) >= 5 * 128 + 5 * 4 and lib.slim_linear8_workspace_bytes(0, 64, 100) == 0
+    assert lib.slim_linear8_workspace_bytes(1, 64, 100) == 0              # one launch, tokens quantised on the way
     assert lib.slim_linear8_backward_workspace_bytes(5, 64, 100, 1) >= 2 * 16 * 128 + 5 * 4
     assert lib.slim_linear8_backward_workspace_bytes(5, 64, 100, 0) >= 3 * 16 * 128 + 5 * 4
     assert lib.slim_linear8_backward_workspace_bytes(5, 64, 100, 7) == 0

@@ -293,8 +293,8 @@ def test_wrapper_refusals(ops):
         ops.gemm8_nt(*(torch.zeros(1, 131072, dtype=torch.int8, device=DEV), scale[:1]) * 2)
     with pytest.raises(ValueError, match="codes_t"):
         ops.linear8_backward(torch.randn(4, 300, device=DEV), codes, scale)
-    with pytest.raises(ValueError, match="one device"):
-        ops.linear8_forward(x, codes, scale.clone().cpu().to(DEV), None) if torch.cuda.device_count() > 1 else ops._same_device(x, x.cpu())
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.linear8_forward(x, codes, scale.cpu())
     assert ops.linear8_forward(x[:0], codes, scale).shape == (0, 10)
     assert ops.linear8_backward(torch.randn(0, 10, device=DEV), ops.transpose8(codes, 100), scale).shape == (0, 100)
 
