@@ -7,7 +7,8 @@
 namespace {
 
 constexpr int BLOCK = 512;       // elements that share a pair of scales: eight per lane, one wave
-constexpr int CHUNK = 4 * BLOCK; // elements of a workgroup's step: one block per wave
+constexpr int CHUNK = 4 * BLOCK; // elements of a workgroup of the update: one block per wave
+constexpr int NORM_CHUNK = 8192; // elements of a workgroup's step of the norm
 
 // one launch takes this many tensors: their addresses travel as kernel arguments (4 KB), which a captured graph keeps by
 // value and which needs no staging buffer
@@ -52,33 +53,49 @@ __device__ __forceinline__ void from_f32(float f, float& o) { o = f; }
 __device__ __forceinline__ void from_f32(float f, bf16_t& o) { o = f32_to_bf16(f); }
 __device__ __forceinline__ void from_f32(float f, _Float16& o) { o = (_Float16)f; }
 
-// four consecutive elements from any element-aligned address
-template <typename T>
-struct Packed4 {
-    typedef T vec __attribute__((ext_vector_type(4)));
-    struct __attribute__((packed, aligned(sizeof(T)))) type { vec v; };
+// COUNT consecutive elements from any element-aligned address
+template <typename T, int COUNT>
+struct Packed {
+    typedef T vec __attribute__((ext_vector_type(COUNT)));
 };
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, int64_t valid, float out[4]) {
-    if (valid >= 4) {
-        const typename Packed4<T>::vec v = ((const typename Packed4<T>::type*)p)->v;
+// Every byte is used once and the arrays are larger than the caches: loads and stores that do not stay there (the sum of
+// squares of 512 MB takes 80 us with them and 132 without, which leave dirty lines of earlier kernels to be written back first; the
+// update of 14 adapters of a 4096-wide block with its norm 167 against 191).
+template <int COUNT, typename T>
+__device__ __forceinline__ typename Packed<T, COUNT>::vec stream_load(const T* p) {
+    typedef typename Packed<T, COUNT>::vec vec;
+    typedef vec unaligned __attribute__((aligned(sizeof(T))));
+    return __builtin_nontemporal_load((const unaligned*)p);
+}
+template <int COUNT, typename T>
+__device__ __forceinline__ void stream_store(T* p, typename Packed<T, COUNT>::vec v) {
+    typedef typename Packed<T, COUNT>::vec vec;
+    typedef vec unaligned __attribute__((aligned(sizeof(T))));
+    __builtin_nontemporal_store(v, (unaligned*)p);
+}
+template <int COUNT, typename T>
+__device__ __forceinline__ void load_run(const T* p, int64_t valid, float out[COUNT]) {
+    if (valid >= COUNT) {
+        const typename Packed<T, COUNT>::vec v = stream_load<COUNT>(p);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) out[j] = to_f32((T)v[j]);
+        for (int j = 0; j < COUNT; ++j) out[j] = to_f32((T)v[j]);
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) out[j] = j < valid ? to_f32(p[j]) : 0.f;
+        for (int j = 0; j < COUNT; ++j) out[j] = j < valid ? to_f32(p[j]) : 0.f;
     }
 }
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, int64_t valid, float out[4]) { load_run<4>(p, valid, out); }
 template <typename T>
 __device__ __forceinline__ void store4(T* p, int64_t valid, const float in[4]) {
     T o[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) from_f32(in[j], o[j]);
     if (valid >= 4) {
-        typename Packed4<T>::vec v;
+        typename Packed<T, 4>::vec v;
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = o[j];
-        ((typename Packed4<T>::type*)p)->v = v;
+        stream_store<4>(p, v);
     } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -86,17 +103,17 @@ __device__ __forceinline__ void store4(T* p, int64_t valid, const float in[4]) {
     }
 }
 __device__ __forceinline__ uint32_t load4_codes(const uint8_t* p, int64_t valid) {
-    struct __attribute__((packed, aligned(1))) word { uint32_t v; };
-    if (valid >= 4) return ((const word*)p)->v;
+    typedef uint32_t word __attribute__((aligned(1)));
+    if (valid >= 4) return __builtin_nontemporal_load((const word*)p);
     uint32_t v = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) v |= (j < valid ? (uint32_t)p[j] : 0u) << (8 * j);
     return v;
 }
 __device__ __forceinline__ void store4_codes(uint8_t* p, int64_t valid, uint32_t c) {
-    struct __attribute__((packed, aligned(1))) word { uint32_t v; };
+    typedef uint32_t word __attribute__((aligned(1)));
     if (valid >= 4) {
-        ((word*)p)->v = c;
+        __builtin_nontemporal_store(c, (word*)p);
         return;
     }
 #pragma unroll
@@ -118,27 +135,41 @@ __device__ __forceinline__ int tensor_of(const uint32_t* first, int count, uint3
 // ---- sqrt(sum of squares) -------------------------------------------------------------------------------------------
 // Squares and sums in 64 bits: the sum runs over up to 10^10 elements, and the update's clipping factor, which it decides, should
 // not depend on how the elements were dealt out.  Partial sums are added in a fixed order.
+// A workgroup takes NORM_CHUNK elements at a time, sixteen bytes per load and four loads per thread under way.
 template <typename T>
 __global__ __launch_bounds__(256) void sumsq_kernel(const NormArgs a, double* __restrict__ part) {
+    constexpr int V = 16 / sizeof(T), U = NORM_CHUNK / (256 * V);
     __shared__ double ws[4];
-    double sum = 0.0;
+    double sum[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) sum[u] = 0.0;
     for (uint32_t c = blockIdx.x; c < a.first[a.count]; c += gridDim.x) {
         const int t = tensor_of(a.first, a.count, c);
-        const int64_t base = (int64_t)(c - a.first[t]) * CHUNK, n = a.n[t];
+        const int64_t base = (int64_t)(c - a.first[t]) * NORM_CHUNK, n = a.n[t];
         const T* g = (const T*)a.g[t];
+        if (n - base >= NORM_CHUNK) {
+            typename Packed<T, V>::vec v[U];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int64_t i = base + (u * 256 + threadIdx.x) * 4;
-            if (i < n) {
-                float x[4];
-                load4(g + i, n - i, x);
+            for (int u = 0; u < U; ++u) v[u] = stream_load<V>(g + base + (u * 256 + threadIdx.x) * V);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) sum += (double)x[j] * (double)x[j];
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const double x = (double)to_f32((T)v[u][j]);
+                    sum[u] = __builtin_fma(x, x, sum[u]);
+                }
+        } else {
+            for (int64_t i = base + threadIdx.x; i < n; i += 256) {
+                const double x = (double)to_f32(g[i]);
+                sum[0] = __builtin_fma(x, x, sum[0]);
             }
         }
     }
-    sum = wave_sum_d(sum);
-    if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = sum;
+    double all = 0.0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) all += sum[u];
+    all = wave_sum_d(all);
+    if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = all;
     __syncthreads();
     if (threadIdx.x == 0) part[blockIdx.x] = (ws[0] + ws[1]) + (ws[2] + ws[3]);
 }
@@ -156,6 +187,7 @@ __global__ __launch_bounds__(256) void norm_kernel(const double* __restrict__ pa
 constexpr int NORM_BLOCKS = 1024;
 
 int64_t chunks_of(int64_t n) { return ceil_div64(n, CHUNK); }
+int64_t norm_chunks_of(int64_t n) { return ceil_div64(n, NORM_CHUNK); }
 
 // ---- the update -----------------------------------------------------------------------------------------------------
 // a 32-bit mix of position and key (multiply and xor-shift, twice); its halves are the random numbers of the two moments
@@ -168,15 +200,22 @@ __device__ __forceinline__ uint32_t mix(uint32_t i, uint32_t key) {
     return h ^ (h >> 16);
 }
 
-// The code of t in [0, largest number] in a float format with MANT mantissa bits and smallest normal number 2^EMIN, rounded up
-// with the probability of t's place between its neighbours: 16 random bits are added below the last kept bit.
-template <int MANT, int EMIN>
-__device__ __forceinline__ uint32_t encode(float t, uint32_t r16) {
-    constexpr int DROP = 23 - MANT;
-    const uint32_t normal = ((f32_bits(t) + (r16 << (DROP - 16))) >> DROP) - ((uint32_t)(EMIN + 126) << MANT);
-    const float unit = __builtin_ldexpf(1.f, MANT - EMIN + 16);
-    const uint32_t small = ((uint32_t)fminf(t * unit, 0x1p24f) + r16) >> 16;
-    return t >= __builtin_ldexpf(1.f, EMIN) ? normal : small;
+// Four codes of float formats of eight bits (e4m3, or e5m2 of numbers >= 0), each rounded up with the probability of its value's
+// place between its neighbours: the conversion adds the seed's high bits below the last bit it keeps; sixteen of them are random
+// (compared with the same sum in integer arithmetic for 16 million values of either format, subnormals among them).
+__device__ __forceinline__ uint32_t encode_e4m3(const float t[4], const uint32_t h[4]) {
+    uint32_t c = 0;
+    c = __builtin_amdgcn_cvt_sr_fp8_f32(t[0], h[0] << 16, c, 0);
+    c = __builtin_amdgcn_cvt_sr_fp8_f32(t[1], h[1] << 16, c, 1);
+    c = __builtin_amdgcn_cvt_sr_fp8_f32(t[2], h[2] << 16, c, 2);
+    return __builtin_amdgcn_cvt_sr_fp8_f32(t[3], h[3] << 16, c, 3);
+}
+__device__ __forceinline__ uint32_t encode_e5m2(const float t[4], const uint32_t h[4]) {
+    uint32_t c = 0;
+    c = __builtin_amdgcn_cvt_sr_bf8_f32(t[0], h[0] & 0xffff0000u, c, 0);
+    c = __builtin_amdgcn_cvt_sr_bf8_f32(t[1], h[1] & 0xffff0000u, c, 1);
+    c = __builtin_amdgcn_cvt_sr_bf8_f32(t[2], h[2] & 0xffff0000u, c, 2);
+    return __builtin_amdgcn_cvt_sr_bf8_f32(t[3], h[3] & 0xffff0000u, c, 3);
 }
 
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
@@ -202,21 +241,12 @@ __device__ __forceinline__ Scale scale_for(uint32_t max_bits, float top) {
 // consecutive elements, four per lane at a time, everything in registers between one read and one write.  The moments follow
 // the formula's fp32 operations exactly (their 8-bit codes are compared bit for bit); the quotient and the root of the update
 // itself are the 1-ulp hardware ones.
-template <typename T, bool EIGHT, bool MASTER>
-__global__ __launch_bounds__(256) void adamw_kernel(const StepArgs a) {
-    const uint32_t c = blockIdx.x;
-    const int t = tensor_of(a.first, a.count, c);
-    const int64_t n = a.n[t];
+template <typename T, bool EIGHT, bool MASTER, bool FULL>
+__device__ __forceinline__ void adamw_block(const StepArgs& a, int t, int64_t block, int64_t n, float clip) {
     const int lane = threadIdx.x & 63;
-    const int64_t block = (int64_t)(c - a.first[t]) * 4 + (threadIdx.x >> 6), base = block * BLOCK;
-    if (base >= n) return;
+    const int64_t base = block * BLOCK;
     T* const p = (T*)a.p[t];
     const T* const g = (const T*)a.g[t];
-    float clip = 1.f;
-    if (a.norm) {
-        const double q = a.max_norm / ((double)a.norm[0] + 1e-6);
-        clip = q < 1.0 || q != q ? (float)q : 1.f;
-    }
     float scale_m = 1.f, scale_v = 1.f;
     if (EIGHT) {
         scale_m = a.s[t][2 * block];
@@ -226,7 +256,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(const StepArgs a) {
     uint32_t top_m = 0, top_v = 0;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        const int64_t i = base + u * 256 + lane * 4, valid = n - i;
+        const int64_t i = base + u * 256 + lane * 4, valid = FULL ? 4 : n - i;
         load4(g + i, valid, x[u]);
         if (MASTER) load4(a.w[t] + i, valid, w[u]);
         else load4(p + i, valid, w[u]);
@@ -250,47 +280,59 @@ __global__ __launch_bounds__(256) void adamw_kernel(const StepArgs a) {
             v[u][j] = v[u][j] * a.b2 + (d * d) * a.c2;
             const float denominator = __builtin_amdgcn_sqrtf(v[u][j]) * a.root + a.eps;
             w[u][j] = w[u][j] * a.keep - (m[u][j] * __builtin_amdgcn_rcpf(denominator)) * a.rate;
-            if (EIGHT) {
-                const bool in = base + u * 256 + lane * 4 + j < n;       // elements behind the last decide no scale
-                top_m = max(top_m, in ? f32_bits(m[u][j]) & 0x7fffffffu : 0u);
-                top_v = max(top_v, in ? f32_bits(v[u][j]) & 0x7fffffffu : 0u);
+            if (EIGHT) {                                 // (elements behind the last were read as zeros and stay zeros)
+                top_m = max(top_m, f32_bits(m[u][j]) & 0x7fffffffu);
+                top_v = max(top_v, f32_bits(v[u][j]) & 0x7fffffffu);
             }
         }
-    Scale sm, sv;
-    uint32_t key = 0;
-    if (EIGHT) {
-        sm = scale_for(wave_max_u32(top_m), 448.f);
-        sv = scale_for(wave_max_u32(top_v), 57344.f);
-        if (lane == 0) {
-            a.s[t][2 * block] = sm.scale;
-            a.s[t][2 * block + 1] = sv.scale;
-        }
-        key = a.seed * 0x85ebca6bu + (uint32_t)(a.index0 + t) * 0xc2b2ae35u + 0x27d4eb2fu;
-    }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        const int64_t i = base + u * 256 + lane * 4, valid = n - i;
+        const int64_t i = base + u * 256 + lane * 4, valid = FULL ? 4 : n - i;
         store4(p + i, valid, w[u]);
         if (MASTER) store4(a.w[t] + i, valid, w[u]);
-        if (EIGHT) {
-            uint32_t cm = 0, cv = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t h = mix((uint32_t)i + j, key);
-                uint32_t em = sm.none ? 0u : encode<3, -6>(fminf(fabsf(m[u][j]) * sm.inverse, 448.f), h & 0xffffu);
-                uint32_t ev = sv.none ? 0u : encode<2, -14>(fminf(v[u][j] * sv.inverse, 57344.f), h >> 16);
-                if (m[u][j] < 0.f) em |= 0x80u;
-                if (!sv.none && ev == 0u && v[u][j] > 0.f) ev = 1u;      // a positive second moment never becomes zero
-                cm |= em << (8 * j);
-                cv |= ev << (8 * j);
-            }
-            store4_codes((uint8_t*)a.m[t] + i, valid, cm);
-            store4_codes((uint8_t*)a.v[t] + i, valid, cv);
-        } else {
+        if (!EIGHT) {
             store4((float*)a.m[t] + i, valid, m[u]);
             store4((float*)a.v[t] + i, valid, v[u]);
         }
     }
+    if (EIGHT) {
+        const Scale sm = scale_for(wave_max_u32(top_m), 448.f), sv = scale_for(wave_max_u32(top_v), 57344.f);
+        if (lane == 0) {
+            a.s[t][2 * block] = sm.scale;
+            a.s[t][2 * block + 1] = sv.scale;
+        }
+        const uint32_t key = a.seed * 0x85ebca6bu + (uint32_t)(a.index0 + t) * 0xc2b2ae35u + 0x27d4eb2fu;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int64_t i = base + u * 256 + lane * 4, valid = FULL ? 4 : n - i;
+            float tm[4], tv[4];
+            uint32_t h[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                h[j] = mix((uint32_t)i + j, key);
+                tm[j] = sm.none ? 0.f : fminf(fmaxf(m[u][j] * sm.inverse, -448.f), 448.f);
+                // a positive second moment never becomes zero: below the smallest number it is that number
+                tv[j] = sv.none || v[u][j] == 0.f ? 0.f : fminf(fmaxf(v[u][j] * sv.inverse, 0x1p-16f), 57344.f);
+            }
+            store4_codes((uint8_t*)a.m[t] + i, valid, encode_e4m3(tm, h));
+            store4_codes((uint8_t*)a.v[t] + i, valid, encode_e5m2(tv, h));
+        }
+    }
+}
+
+template <typename T, bool EIGHT, bool MASTER>
+__global__ __launch_bounds__(256) void adamw_kernel(const StepArgs a) {
+    const uint32_t c = blockIdx.x;
+    const int t = tensor_of(a.first, a.count, c);
+    const int64_t n = a.n[t], block = (int64_t)(c - a.first[t]) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (block * BLOCK >= n) return;
+    float clip = 1.f;
+    if (a.norm) {
+        const double q = a.max_norm / ((double)a.norm[0] + 1e-6);
+        clip = q < 1.0 || q != q ? (float)q : 1.f;
+    }
+    if (n - block * BLOCK >= BLOCK) adamw_block<T, EIGHT, MASTER, true>(a, t, block, n, clip);
+    else adamw_block<T, EIGHT, MASTER, false>(a, t, block, n, clip);
 }
 
 template <typename T>
@@ -330,11 +372,11 @@ extern "C" int slim_grad_norm(const void* const* grads, const int64_t* numel, in
     for (int i = 0; i < count;) {
         NormArgs a;
         int64_t chunks = 0;
-        for (a.count = 0; a.count < NORM_TENSORS && i < count && chunks + chunks_of(numel[i]) <= MAX_CHUNKS; ++a.count, ++i) {
+        for (a.count = 0; a.count < NORM_TENSORS && i < count && chunks + norm_chunks_of(numel[i]) <= MAX_CHUNKS; ++a.count, ++i) {
             a.g[a.count] = grads[i];
             a.n[a.count] = numel[i];
             a.first[a.count] = (uint32_t)chunks;
-            chunks += chunks_of(numel[i]);
+            chunks += norm_chunks_of(numel[i]);
         }
         a.first[a.count] = (uint32_t)chunks;
         const int blocks = (int)(chunks < NORM_BLOCKS ? chunks : NORM_BLOCKS);

@@ -105,8 +105,10 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
     auto fetch = [&](int64_t c, float v[8]) {
         load8(src + c, K - c, v);
         if (PLANES > 1) {
+            float f[8];
+            load8(colscale + c, K - c, f);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = c + j < K ? v[j] * colscale[c + j] : 0.f;
+            for (int j = 0; j < 8; ++j) v[j] *= f[j];
         }
     };
     auto take = [&](const float v[8]) {
