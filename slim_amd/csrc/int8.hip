@@ -28,10 +28,12 @@ struct Packed8 {
     typedef T vec __attribute__((ext_vector_type(8)));
     struct __attribute__((packed, aligned(sizeof(T)))) type { vec v; };
 };
-template <typename T>
+// (ONCE: data that is not read again and need not stay in the caches)
+template <bool ONCE = false, typename T>
 __device__ __forceinline__ void load8(const T* p, int64_t valid, float out[8]) {
     if (valid >= 8) {
-        const typename Packed8<T>::vec v = ((const typename Packed8<T>::type*)p)->v;
+        typedef typename Packed8<T>::vec unaligned __attribute__((aligned(sizeof(T))));
+        const typename Packed8<T>::vec v = ONCE ? __builtin_nontemporal_load((const unaligned*)p) : ((const typename Packed8<T>::type*)p)->v;
 #pragma unroll
         for (int j = 0; j < 8; ++j) out[j] = to_f32((T)v[j]);
     } else {
@@ -88,7 +90,8 @@ __device__ __forceinline__ void store_codes(const float x[8], float r, int8_t* c
 }
 
 // WPR waves work on a row (four rows per workgroup, or one); each thread keeps NV pieces of eight elements in registers, so
-// the row is read once.  NV = 0: rows too long for that are read twice.
+// the row is read once, with loads that do not stay in the caches (28672 x 8192 bf16: 109 us, 6.4 TB/s; 126 without).
+// NV = 0: rows too long for that are read twice.
 template <typename T, int PLANES, int NV, int WPR>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int64_t R, int64_t K, int64_t ldx,
                                                             const float* __restrict__ colscale, int8_t* __restrict__ codes,
@@ -103,7 +106,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
     float keep[NV > 0 ? NV : 1][8];
     uint32_t m = 0;
     auto fetch = [&](int64_t c, float v[8]) {
-        load8(src + c, K - c, v);
+        load8<(NV > 0)>(src + c, K - c, v);
         if (PLANES > 1) {
             float f[8];
             load8(colscale + c, K - c, f);
@@ -214,6 +217,7 @@ struct Gemm8Args {
     int tiles_m, tiles_n;
     int splits, steps_per_split;                         // slices of the reduction, each into a slab of its own
     int32_t* slab;                                       // [splits][tiles_m * BM][tiles_n * BN], or null: one slice, results written here
+    int rest_n;                                          // columns of narrower tiles behind the tiles_n full ones (0: none)
 };
 
 template <int N>
@@ -237,11 +241,19 @@ template <int CNT, typename T, typename F>
 __device__ __forceinline__ void store_row(T* dst, int64_t left, F value) {
     if (left >= CNT) {
 #pragma unroll
-        for (int c = 0; c < CNT; c += 8) {
+        for (int c = 0; c + 8 <= CNT; c += 8) {
             typename Packed8<T>::vec v;
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = value(c + j);
             ((typename Packed8<T>::type*)(dst + c))->v = v;
+        }
+        if (CNT % 8) {
+            typedef T quad __attribute__((ext_vector_type(4)));
+            struct __attribute__((packed, aligned(sizeof(T)))) unaligned { quad v; };
+            quad v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = value(CNT - 4 + j);
+            ((unaligned*)(dst + CNT - 4))->v = v;
         }
     } else {
 #pragma unroll
@@ -253,7 +265,9 @@ __device__ __forceinline__ void store_row(T* dst, int64_t left, F value) {
 template <int CNT, typename T>
 __device__ __forceinline__ void load_run(const T* src, int64_t left, float out[CNT]) {
 #pragma unroll
-    for (int c = 0; c < CNT; c += 8) load8(src + c, left - c, out + c);
+    for (int c = 0; c + 8 <= CNT; c += 8) load8(src + c, left - c, out + c);
+#pragma unroll
+    for (int c = CNT / 8 * 8; c < CNT; ++c) out[c] = c < left ? to_f32(src[c]) : 0.f;
 }
 
 // One value from its planes' sums, the highest plane first.
@@ -265,14 +279,14 @@ __device__ __forceinline__ float join_planes(const int* sums, int stride) {
     return v;
 }
 
-// The workgroup's tile and slice.  Workgroups go to the eight XCDs in turn; each XCD gets a run of consecutive tiles, and a run
-// walks groups of eight rows of tiles column by column, so that the 32 workgroups of an XCD share 8 panels of A and 4 of B in
-// its L2 (4096 x 11008 x 4096 on the 256 x 256 tile: 159 us, with groups of four 171 us).
-__device__ __forceinline__ void tile_of(const Gemm8Args& g, int& tm, int& tn, int& slice) {
-    const int per = g.tiles_m * g.tiles_n, total = per * g.splits, b = blockIdx.x, x = b & 7, share = total >> 3, rest = total & 7;
+// Tile and slice of workgroup b of tiles_m * tiles_n * splits.  Workgroups go to the eight XCDs in turn; each XCD gets a run of
+// consecutive tiles, and a run walks groups of eight rows of tiles column by column, so that the 32 workgroups of an XCD share 8
+// panels of A and 4 of B in its L2 (4096 x 11008 x 4096 on the 256 x 256 tile: 159 us, with groups of four 171 us).
+__device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int splits, int& tm, int& tn, int& slice) {
+    const int per = tiles_m * tiles_n, total = per * splits, x = b & 7, share = total >> 3, rest = total & 7;
     const int t = x * share + min(x, rest) + (b >> 3);
     slice = t / per;
-    const int u = t - slice * per, group = u / (8 * g.tiles_n), m0 = group * 8, gm = min(8, g.tiles_m - m0), r = u - group * 8 * g.tiles_n;
+    const int u = t - slice * per, group = u / (8 * tiles_n), m0 = group * 8, gm = min(8, tiles_m - m0), r = u - group * 8 * tiles_n;
     tm = m0 + r % gm;
     tn = r / gm;
 }
@@ -291,21 +305,15 @@ __device__ __forceinline__ void tile_of(const Gemm8Args& g, int& tm, int& tn, in
 // Whole 128-byte lines per row: with 64-byte steps, which would allow four stages, the requests take twice as long (171 us).
 // What bounds it: without requests the loop takes 138 us, without fragment reads as well 123 us; the matrix instructions alone hold
 // the clock at about 2.1 GHz.
-template <int PLANES, int FM, int FN, int WM, int WN, int STAGES, int OCC>
-__global__ __launch_bounds__(64 * WM * WN, OCC) void gemm8_kernel(const Gemm8Args g) {
+template <int PLANES, int FM, int FN, int WM, int WN, int STAGES>
+__device__ __forceinline__ void gemm8_tile(const Gemm8Args& g, char* lds, int64_t row0, int64_t col0, int slice) {
     constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN, NW = WM * WN;
     constexpr int PIECES = (BM + BN) / 8, PPW = (PIECES + NW - 1) / NW;     // (a last wave repeats the final piece)
     constexpr int STAGE_BYTES = (BM + BN) * 128;
     constexpr int RUN = 4 * FN;                          // consecutive columns of a lane
-    constexpr int KB = FN == 8 ? 5 : FN == 4 ? 4 : FN == 2 ? 3 : 2;      // the bit of a B row that tells lane rows r and r + 4 apart
     constexpr int READS = FM + FN, PRODUCTS = FM * FN;
     constexpr int PACE1 = PRODUCTS / READS > 0 ? PRODUCTS / READS : 1, PACE2 = PRODUCTS / (READS + PPW) > 0 ? PRODUCTS / (READS + PPW) : 1;
     static_assert(FM % PLANES == 0, "a wave holds whole groups of planes");
-    
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    int tm, tn, slice;
-    tile_of(g, tm, tn, slice);
-    const int64_t row0 = (int64_t)tm * BM, col0 = (int64_t)tn * BN;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave / WN, wc = wave % WN;
     const int fr = lane & 15, fq = lane >> 4;
@@ -329,7 +337,7 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm8_kernel(const Gemm8Arg
                 base[s] = g.A + row0 * g.lda;
                 off[s] = (uint32_t)(min((int64_t)R, g.rows - 1 - row0) * g.lda) + (pc ^ (R & 7)) * 16;
             } else {
-                const int R = q * 8 - BM + pr, key = (R & 3) | (((R >> KB) & 1) << 2);
+                const int R = q * 8 - BM + pr, key = (R & 3) | (((R / RUN) & 1) << 2);
                 base[s] = g.B + col0 * g.ldb;
                 off[s] = (uint32_t)(min((int64_t)R, g.N - 1 - col0) * g.ldb) + (pc ^ key) * 16;
             }
@@ -443,6 +451,24 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm8_kernel(const Gemm8Arg
     }
 }
 
+// REST > 0: behind the columns of full tiles lie g.rest_n columns of tiles of 16 REST WN columns (the last round of workgroups).
+template <int PLANES, int FM, int FN, int WM, int WN, int STAGES, int OCC, int REST>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void gemm8_kernel(const Gemm8Args g) {
+    constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    int tm, tn, slice;
+    if constexpr (REST > 0) {
+        const int full = g.tiles_m * g.tiles_n;
+        if ((int)blockIdx.x >= full) {
+            tile_of((int)blockIdx.x - full, g.tiles_m, g.rest_n, 1, tm, tn, slice);
+            gemm8_tile<PLANES, FM, REST, WM, WN, STAGES>(g, lds, (int64_t)tm * BM, (int64_t)g.tiles_n * BN + (int64_t)tn * 16 * REST * WN, 0);
+            return;
+        }
+    }
+    tile_of(blockIdx.x, g.tiles_m, g.tiles_n, g.splits, tm, tn, slice);
+    gemm8_tile<PLANES, FM, FN, WM, WN, STAGES>(g, lds, (int64_t)tm * BM, (int64_t)tn * BN, slice);
+}
+
 // The slices' sums added (whole numbers: any order gives the same), planes joined, scaled and rounded: a thread per four columns.
 template <int PLANES>
 __global__ __launch_bounds__(256) void join_slices_kernel(const Gemm8Args g, int64_t slab_rows, int64_t slab_cols) {
@@ -492,6 +518,8 @@ struct Tiles<3> {                                        // (a wave's rows are a
 struct Plan {
     int tile = 0, splits = 1, steps_per_split = 0;
     int64_t tiles_m = 0, tiles_n = 0, slab_rows = 0, slab_cols = 0;
+    int rest = 0;                                        // fragments (of 64 columns) of the narrower tiles behind the full ones
+    int64_t rest_n = 0;
     int64_t slab_bytes() const { return splits > 1 ? splits * slab_rows * slab_cols * 4 : 0; }
 };
 template <int PLANES>
@@ -517,16 +545,28 @@ Plan plan_gemm8(int64_t rows, int64_t N, int64_t steps) {
             }
         }
     }
+    // The largest tile's last round, when it is not full, on narrower tiles that fill it better (4096 x 11008: 512 full tiles and 240 of
+    // 192 columns in place of 176 full ones).
+    if (PLANES < 3 && best.tile == 0 && best.splits == 1 && best.tiles_m <= 256) {
+        const int64_t tiles = best.tiles_m * best.tiles_n, columns = tiles / 256 * 256 / best.tiles_m;
+        if (tiles > 256 && tiles % 256 && columns < best.tiles_n) {
+            for (int rest = 3; rest >= 2; --rest) {
+                const int64_t n = ceil_div64(N - columns * 256, 64 * rest);
+                if (columns * best.tiles_m + n * best.tiles_m <= (tiles / 256 + 1) * 256) best.rest = rest, best.rest_n = n;
+            }
+            if (best.rest) best.tiles_n = columns;
+        }
+    }
     return best;
 }
 
-template <int PLANES, int TILE, int FM, int FN, int WM, int WN, int STAGES, int OCC>
+template <int PLANES, int TILE, int FM, int FN, int WM, int WN, int STAGES, int OCC, int REST = 0>
 int launch_gemm8(const Gemm8Args& g, const Plan& p, hipStream_t st) {
     constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN, bytes = STAGES * (BM + BN) * 128;
-    const int64_t blocks = p.tiles_m * p.tiles_n * p.splits;
+    const int64_t blocks = p.tiles_m * p.tiles_n * p.splits + p.tiles_m * p.rest_n;
     static_assert(Tiles<PLANES>::list[TILE].bm == BM && Tiles<PLANES>::list[TILE].bn == BN, "the plan's tile");
     SLIM_REQUIRE(blocks * 64 * WM * WN < (int64_t)1 << 32 && blocks < 0x7fffffff, "gemm8: the result is too large for one launch");
-    auto kernel = gemm8_kernel<PLANES, FM, FN, WM, WN, STAGES, OCC>;
+    auto kernel = gemm8_kernel<PLANES, FM, FN, WM, WN, STAGES, OCC, REST>;
     SLIM_HIP(slim_allow_dynamic_lds((const void*)kernel, bytes));
     kernel<<<(unsigned)blocks, 64 * WM * WN, bytes, st>>>(g);
     SLIM_LAUNCH_CHECK();
@@ -539,13 +579,15 @@ int gemm8(Gemm8Args g, void* slab, hipStream_t st) {
               2.0 * g.rows * g.N * g.steps * 128);
     const Plan p = plan_gemm8<PLANES>(g.rows, g.N, g.steps);
     g.tiles_m = (int)p.tiles_m, g.tiles_n = (int)p.tiles_n;
-    g.splits = p.splits, g.steps_per_split = p.steps_per_split;
+    g.splits = p.splits, g.steps_per_split = p.steps_per_split, g.rest_n = (int)p.rest_n;
     g.slab = p.splits > 1 ? (int32_t*)slab : nullptr;
     int rc;
     if constexpr (PLANES == 3) {
         rc = p.tile == 0 ? launch_gemm8<3, 0, 6, 4, 2, 4, 2, 2>(g, p, st) : launch_gemm8<3, 1, 3, 2, 2, 4, 4, 2>(g, p, st);
     } else {
-        if (p.tile == 0) rc = launch_gemm8<PLANES, 0, 8, 4, 2, 4, 2, 2>(g, p, st);
+        if (p.tile == 0 && p.rest == 3) rc = launch_gemm8<PLANES, 0, 8, 4, 2, 4, 2, 2, 3>(g, p, st);
+        else if (p.tile == 0 && p.rest == 2) rc = launch_gemm8<PLANES, 0, 8, 4, 2, 4, 2, 2, 2>(g, p, st);
+        else if (p.tile == 0) rc = launch_gemm8<PLANES, 0, 8, 4, 2, 4, 2, 2>(g, p, st);
         else if (p.tile == 1) rc = launch_gemm8<PLANES, 1, 4, 4, 2, 4, 3, 2>(g, p, st);
         else if (p.tile == 2) rc = launch_gemm8<PLANES, 2, 4, 2, 2, 4, 4, 2>(g, p, st);
         else rc = launch_gemm8<PLANES, 3, 2, 2, 2, 4, 3, 4>(g, p, st);
@@ -885,7 +927,7 @@ extern "C" int slim_gemm8_nt(const int8_t* a, int64_t lda, const float* sa, cons
                  "slim_gemm8_nt: workspace too small or misaligned");
     SLIM_REQUIRE(lda < 1 << 23 && ldb < 1 << 23, "slim_gemm8_nt: rows of codes lie too far apart");
     if (takes_ring(M, N)) return launch_ring8(RingArgs{a, lda, sa, b, ldb, sb, bias, out, ldo, dtype, (int)M, (int)N, (int)(pad128(K) / 128)}, (hipStream_t)stream);
-    Gemm8Args g{a, b, lda, ldb, M, M, N, (int)(pad128(K) / 128), sa, sb, bias, out, ldo, dtype, 0, 0, 1, 0, nullptr};
+    Gemm8Args g{a, b, lda, ldb, M, M, N, (int)(pad128(K) / 128), sa, sb, bias, out, ldo, dtype, 0, 0, 1, 0, nullptr, 0};
     return gemm8<1>(g, workspace, (hipStream_t)stream);
 }
 
@@ -938,6 +980,6 @@ extern "C" int slim_linear8_backward(const void* dy, int dtype, int64_t lddy, in
                                : quantize_rows_any<2>(dy, dtype, M, N, lddy, scale, q, ld, sq, st);
     if (rc) return rc;
     void* slab = (char*)sq + align256(M * 4);
-    Gemm8Args g{q, codes_t, ld, ld, rows, M, K, (int)(ld / 128), sq, nullptr, nullptr, dx, lddx, dtype, 0, 0, 1, 0, nullptr};
+    Gemm8Args g{q, codes_t, ld, ld, rows, M, K, (int)(ld / 128), sq, nullptr, nullptr, dx, lddx, dtype, 0, 0, 1, 0, nullptr, 0};
     return planes == 3 ? gemm8<3>(g, slab, st) : gemm8<2>(g, slab, st);
 }

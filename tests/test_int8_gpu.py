@@ -122,6 +122,34 @@ def test_product_against_64_bits(ops, M, N, K, dtype):
         assert within(out, p, bound(p, bias, dtype), dtype), float(((out - p).abs() - bound(p, bias, dtype)).max())
 
 
+# every tile and its neighbours: 256 x 256 alone, with a last round of 192 and of 128 columns, 128 x 256, 128 x 128, 64 x 128, and slices of
+# the reduction (4 and 8); ragged in both directions.  The reference product runs on the GPU in 64 bits (whole numbers: exact).
+LARGE = [(2500, 4099, 200), (2048, 4095, 500), (6000, 4097, 700), (4100, 4100, 300), (2049, 4097, 500), (513, 5121, 13000), (1111, 2222, 1000), (70, 130, 20000), (300, 201, 13000), (90, 9001, 5000)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", LARGE)
+def test_large_products_against_64_bits(ops, M, N, K, dtype):
+    a, b = random_codes(M, K, 1).to(DEV), random_codes(N, K, 2).to(DEV)
+    sa, sb = torch.rand(M, device=DEV) * 1e-2, torch.rand(N, device=DEV) * 1e-2
+    bias = torch.randn(N, device=DEV).to(dtype)
+    out = ops.gemm8_nt(a, sa, b, sb, bias, dtype).double()
+    p = (a.double() @ b.double().t()) * sa.double()[:, None] * sb.double() + bias.double()
+    assert within(out, p, bound(p, bias, dtype), dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(2100, 300, 4101), (4101, 300, 5003), (3100, 200, 4097), (1025, 1000, 2100), (513, 5000, 1100), (40, 20001, 131), (17, 13001, 200)])
+def test_large_gradients_against_64_bits(ops, M, N, K, dtype):
+    w = random_codes(N, K, 3).to(DEV)
+    g = torch.Generator(device=DEV).manual_seed(4)
+    scale = torch.rand(N, generator=g, device=DEV) * 1e-2
+    dy = torch.randn(M, N, generator=g, device=DEV).to(dtype)
+    dx = ops.linear8_backward(dy, ops.transpose8(w, K), scale).double()
+    exact, allowed = gradient_bound(dy, w[:, :K], scale, dtype)
+    assert bool(((dx - exact).abs() <= allowed).all()), float(((dx - exact).abs() / allowed).max())
+
+
 def test_longest_sum_is_exact(ops):
     """131071 products of -128 by -128: 2^31 - 16384, the largest sum 32 bits have to hold."""
     K = 131071
