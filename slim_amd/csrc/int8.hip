@@ -4,6 +4,7 @@
 // floating-point products (slim/quantization/quantization.py:219-263, :266-304).
 #include "common.hpp"
 #include "../../include/slim_hip.h"
+#include <type_traits>
 
 namespace {
 
@@ -236,38 +237,30 @@ __device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float v)
     else ((_Float16*)p)[i] = (_Float16)v;
 }
 
-// CNT consecutive results of one row, from any element-aligned address
+// CNT (8 or 4) consecutive results of one row, to any element-aligned address
 template <int CNT, typename T, typename F>
-__device__ __forceinline__ void store_row(T* dst, int64_t left, F value) {
+__device__ __forceinline__ void store_run(T* dst, int64_t left, F value) {
     if (left >= CNT) {
+        typedef T vec __attribute__((ext_vector_type(CNT)));
+        struct __attribute__((packed, aligned(sizeof(T)))) unaligned { vec v; };
+        vec v;
 #pragma unroll
-        for (int c = 0; c + 8 <= CNT; c += 8) {
-            typename Packed8<T>::vec v;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = value(c + j);
-            ((typename Packed8<T>::type*)(dst + c))->v = v;
-        }
-        if (CNT % 8) {
-            typedef T quad __attribute__((ext_vector_type(4)));
-            struct __attribute__((packed, aligned(sizeof(T)))) unaligned { quad v; };
-            quad v;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = value(CNT - 4 + j);
-            ((unaligned*)(dst + CNT - 4))->v = v;
-        }
+        for (int j = 0; j < CNT; ++j) v[j] = value(j);
+        ((unaligned*)dst)->v = v;
     } else {
 #pragma unroll
         for (int j = 0; j < CNT; ++j)
             if (j < left) dst[j] = value(j);
     }
 }
-
 template <int CNT, typename T>
-__device__ __forceinline__ void load_run(const T* src, int64_t left, float out[CNT]) {
+__device__ __forceinline__ void load_run(const T* src, int64_t left, float* out) {
+    if constexpr (CNT == 8) {
+        load8(src, left, out);
+    } else {
 #pragma unroll
-    for (int c = 0; c + 8 <= CNT; c += 8) load8(src + c, left - c, out + c);
-#pragma unroll
-    for (int c = CNT / 8 * 8; c < CNT; ++c) out[c] = c < left ? to_f32(src[c]) : 0.f;
+        for (int c = 0; c < CNT; ++c) out[c] = c < left ? to_f32(src[c]) : 0.f;
+    }
 }
 
 // One value from its planes' sums, the highest plane first.
@@ -310,7 +303,7 @@ __device__ __forceinline__ void gemm8_tile(const Gemm8Args& g, char* lds, int64_
     constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN, NW = WM * WN;
     constexpr int PIECES = (BM + BN) / 8, PPW = (PIECES + NW - 1) / NW;     // (a last wave repeats the final piece)
     constexpr int STAGE_BYTES = (BM + BN) * 128;
-    constexpr int RUN = 4 * FN;                          // consecutive columns of a lane
+    constexpr int PAIRS = FN / 2 * 32;                   // columns (rows of B) of a wave's fragments taken in pairs
     constexpr int READS = FM + FN, PRODUCTS = FM * FN;
     constexpr int PACE1 = PRODUCTS / READS > 0 ? PRODUCTS / READS : 1, PACE2 = PRODUCTS / (READS + PPW) > 0 ? PRODUCTS / (READS + PPW) : 1;
     static_assert(FM % PLANES == 0, "a wave holds whole groups of planes");
@@ -337,7 +330,7 @@ __device__ __forceinline__ void gemm8_tile(const Gemm8Args& g, char* lds, int64_
                 base[s] = g.A + row0 * g.lda;
                 off[s] = (uint32_t)(min((int64_t)R, g.rows - 1 - row0) * g.lda) + (pc ^ (R & 7)) * 16;
             } else {
-                const int R = q * 8 - BM + pr, key = (R & 3) | (((R / RUN) & 1) << 2);
+                const int R = q * 8 - BM + pr, w = R % (16 * FN), key = w < PAIRS ? (w & 3) | (((w >> 3) & 1) << 2) : w & 7;
                 base[s] = g.B + col0 * g.ldb;
                 off[s] = (uint32_t)(min((int64_t)R, g.N - 1 - col0) * g.ldb) + (pc ^ key) * 16;
             }
@@ -354,13 +347,15 @@ __device__ __forceinline__ void gemm8_tile(const Gemm8Args& g, char* lds, int64_
     for (int st = 0; st < STAGES; ++st) request(st, st);
     const int x0 = (fq ^ (fr & 7)) * 16;
     const int a_off = (wr * 16 * FM + fr) * 128 + x0;
-    const int b_off = (BM + wc * 16 * FN + (fr >> 2) * RUN + (fr & 3)) * 128 + x0;
+    const int b_off = (BM + wc * 16 * FN + (fr >> 2) * 8 + (fr & 3)) * 128 + x0;
+    const int odd_off = (BM + wc * 16 * FN + PAIRS + fr) * 128 + x0;     // the last fragment of an odd number
     i32x4 af[2][FM], bf[2][FN];
     auto read = [&](int half, int stage) {
         const char* a = lds + ((stage * STAGE_BYTES + a_off) ^ (half * 64));
         const char* b = lds + ((stage * STAGE_BYTES + b_off) ^ (half * 64));
 #pragma unroll
-        for (int j = 0; j < FN; ++j) bf[half][j] = *(const i32x4*)(b + j * 4 * 128);
+        for (int j = 0; j < FN / 2 * 2; ++j) bf[half][j] = *(const i32x4*)(b + ((j >> 1) * 32 + (j & 1) * 4) * 128);
+        if (FN % 2) bf[half][FN - 1] = *(const i32x4*)(lds + ((stage * STAGE_BYTES + odd_off) ^ (half * 64)));
 #pragma unroll
         for (int i = 0; i < FM; ++i) af[half][i] = *(const i32x4*)(a + i * 16 * 128);
     };
@@ -410,45 +405,52 @@ __device__ __forceinline__ void gemm8_tile(const Gemm8Args& g, char* lds, int64_
     }
     wait_vmcnt<0>();                                     // (the requests behind the last step land before the LDS is given up)
 
-    const int64_t n0 = col0 + wc * 16 * FN + fq * RUN;
+    const int64_t n0 = col0 + wc * 16 * FN;              // value 8 c + k of a lane: column n0 + 32 c + 8 fq + k, of an odd fragment n0 + PAIRS + 4 fq + k
     if (g.slab) {
         int32_t* slab = g.slab + ((int64_t)slice * g.tiles_m * BM + row0 + wr * 16 * FM + fr) * ((int64_t)g.tiles_n * BN) + n0;
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
-            for (int j = 0; j < FN; ++j) *(i32x4*)(slab + (int64_t)i * 16 * g.tiles_n * BN + 4 * j) = acc[i][j];
+            for (int j = 0; j < FN; ++j)
+                *(i32x4*)(slab + (int64_t)i * 16 * g.tiles_n * BN + (j < FN / 2 * 2 ? (j >> 1) * 32 + fq * 8 + (j & 1) * 4 : PAIRS + fq * 4)) = acc[i][j];
         return;
     }
-    const int64_t left = g.N - n0;
-    if (left <= 0) return;
     // everything the epilogue reads is requested at once (loaded row by row it costs a trip to memory per row: 4 us of a 256 x 256 tile)
     const int64_t group0 = (row0 / 16 + wr * FM) / PLANES;
-    float sa[FM / PLANES], sb[RUN], bias[RUN];
+    float sa[FM / PLANES], sb[4 * FN], bias[4 * FN];
 #pragma unroll
     for (int i = 0; i < FM / PLANES; ++i) sa[i] = g.sa[min((group0 + i) * 16 + fr, g.M - 1)];
 #pragma unroll
-    for (int c = 0; c < RUN; ++c) sb[c] = 1.f, bias[c] = 0.f;
-    if (g.sb) load_run<RUN>(g.sb + n0, left, sb);
+    for (int c = 0; c < 4 * FN; ++c) sb[c] = 1.f, bias[c] = 0.f;
+    auto columns = [&](auto take) {                      // take(first value, how many, column) for each of the lane's runs of columns
+#pragma unroll
+        for (int c = 0; c < FN / 2; ++c) take(std::integral_constant<int, 8>(), c * 8, n0 + c * 32 + fq * 8);
+        if constexpr (FN % 2) take(std::integral_constant<int, 4>(), 4 * FN - 4, n0 + PAIRS + fq * 4);
+    };
+    if (g.sb) columns([&](auto count, int c, int64_t n) { load_run<count.value>(g.sb + n, g.N - n, sb + c); });
     if (g.bias) {
-        if (g.dtype == SLIM_DTYPE_F32) load_run<RUN>((const float*)g.bias + n0, left, bias);
-        else if (g.dtype == SLIM_DTYPE_BF16) load_run<RUN>((const bf16_t*)g.bias + n0, left, bias);
-        else load_run<RUN>((const _Float16*)g.bias + n0, left, bias);
+        if (g.dtype == SLIM_DTYPE_F32) columns([&](auto count, int c, int64_t n) { load_run<count.value>((const float*)g.bias + n, g.N - n, bias + c); });
+        else if (g.dtype == SLIM_DTYPE_BF16) columns([&](auto count, int c, int64_t n) { load_run<count.value>((const bf16_t*)g.bias + n, g.N - n, bias + c); });
+        else columns([&](auto count, int c, int64_t n) { load_run<count.value>((const _Float16*)g.bias + n, g.N - n, bias + c); });
     }
+    auto rows = [&](auto* out, auto convert) {
 #pragma unroll
-    for (int i = 0; i < FM / PLANES; ++i) {
-        const int64_t m = (group0 + i) * 16 + fr;
-        if (m >= g.M) continue;
-        auto value = [&](int c) {
-            int sums[PLANES];
+        for (int i = 0; i < FM / PLANES; ++i) {
+            const int64_t m = (group0 + i) * 16 + fr;
+            if (m >= g.M) continue;
+            auto value = [&](int c) {
+                int sums[PLANES];
 #pragma unroll
-            for (int p = 0; p < PLANES; ++p) sums[p] = acc[i * PLANES + p][c >> 2][c & 3];
-            const float v = (join_planes<PLANES>(sums, 1) * sa[i]) * sb[c];
-            return g.bias ? v + bias[c] : v;
-        };
-        if (g.dtype == SLIM_DTYPE_F32) store_row<RUN>((float*)g.out + m * g.ldo + n0, left, value);
-        else if (g.dtype == SLIM_DTYPE_BF16) store_row<RUN>((bf16_t*)g.out + m * g.ldo + n0, left, [&](int c) { return f32_to_bf16(value(c)); });
-        else store_row<RUN>((_Float16*)g.out + m * g.ldo + n0, left, [&](int c) { return (_Float16)value(c); });
-    }
+                for (int p = 0; p < PLANES; ++p) sums[p] = acc[i * PLANES + p][c >> 2][c & 3];
+                const float v = (join_planes<PLANES>(sums, 1) * sa[i]) * sb[c];
+                return convert(g.bias ? v + bias[c] : v);
+            };
+            columns([&](auto count, int c, int64_t n) { store_run<count.value>(out + m * g.ldo + n, g.N - n, [&](int k) { return value(c + k); }); });
+        }
+    };
+    if (g.dtype == SLIM_DTYPE_F32) rows((float*)g.out, [](float v) { return v; });
+    else if (g.dtype == SLIM_DTYPE_BF16) rows((bf16_t*)g.out, [](float v) { return f32_to_bf16(v); });
+    else rows((_Float16*)g.out, [](float v) { return (_Float16)v; });
 }
 
 // REST > 0: behind the columns of full tiles lie g.rest_n columns of tiles of 16 REST WN columns (the last round of workgroups).
