@@ -90,19 +90,19 @@ __device__ __forceinline__ void store_codes(const float x[8], float r, int8_t* c
     }
 }
 
-// WPR waves work on a row (four rows per workgroup, or one); each thread keeps NV pieces of eight elements in registers, so
+// WPR waves work on a row (one: four rows per workgroup; four or sixteen: one); each thread keeps NV pieces of eight elements in registers, so
 // the row is read once, with loads that do not stay in the caches (28672 x 8192 bf16: 109 us, 6.4 TB/s; 126 without).
 // NV = 0: rows too long for that are read twice.
 template <typename T, int PLANES, int NV, int WPR>
-__global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, int64_t R, int64_t K, int64_t ldx,
+__global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void quantize_rows_kernel(const T* __restrict__ x, int64_t R, int64_t K, int64_t ldx,
                                                             const float* __restrict__ colscale, int8_t* __restrict__ codes,
                                                             int64_t ldc, float* __restrict__ scale) {
     constexpr int TPR = 64 * WPR;                        // threads of a row
-    __shared__ uint32_t part[4];
+    __shared__ uint32_t part[WPR];
     const int wave = threadIdx.x >> 6;
-    const int64_t row = WPR == 4 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+    const int64_t row = WPR > 1 ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
     if (WPR == 1 && row >= R) return;
-    const int t = WPR == 4 ? threadIdx.x : threadIdx.x & 63;
+    const int t = WPR > 1 ? threadIdx.x : threadIdx.x & 63;
     const T* src = x + row * ldx;
     float keep[NV > 0 ? NV : 1][8];
     uint32_t m = 0;
@@ -146,10 +146,11 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
         const uint32_t b = (uint32_t)__shfl_xor((int)m, o, 64);
         m = b > m ? b : m;
     }
-    if (WPR == 4) {
+    if (WPR > 1) {
         if ((threadIdx.x & 63) == 0) part[wave] = m;
         __syncthreads();
-        m = max(max(part[0], part[1]), max(part[2], part[3]));
+#pragma unroll
+        for (int i = 0; i < WPR; ++i) m = max(m, part[i]);
     }
     const RowScale rs = row_scale<PLANES>(m);
     if (t == 0) scale[row] = rs.scale;
@@ -180,15 +181,18 @@ template <typename T, int PLANES>
 int quantize_rows(const T* x, int64_t R, int64_t K, int64_t ldx, const float* colscale, int8_t* codes, int64_t ldc, float* scale,
                   hipStream_t st) {
     const int64_t pieces = (K + 127) / 128 * 16;         // pieces of eight codes in a padded row
+    SLIM_REQUIRE(R * (pieces > 1024 ? 1024 : 256) < (int64_t)1 << 32, "quantize_rows8: too many rows for one launch");
 #define SLIM_ROWS(NV, WPR)                                                                                                  \
-    quantize_rows_kernel<T, PLANES, NV, WPR><<<(unsigned)(WPR == 4 ? R : ceil_div64(R, 4)), 256, 0, st>>>(x, R, K, ldx, colscale, codes, ldc, scale)
+    quantize_rows_kernel<T, PLANES, NV, WPR><<<(unsigned)(WPR > 1 ? R : ceil_div64(R, 4)), WPR == 16 ? 1024 : 256, 0, st>>>(x, R, K, ldx, colscale, codes, ldc, scale)
     if (pieces <= 64) SLIM_ROWS(1, 1);
     else if (pieces <= 128) SLIM_ROWS(2, 1);
     else if (pieces <= 256) SLIM_ROWS(4, 1);
     else if (pieces <= 512) SLIM_ROWS(2, 4);
     else if (pieces <= 1024) SLIM_ROWS(4, 4);
-    else if (pieces <= 2048) SLIM_ROWS(8, 4);
-    else SLIM_ROWS(0, 4);
+    else if (pieces <= 2048 && R >= 4096) SLIM_ROWS(8, 4);             // (8192 x 13824 bf16: 63 us, with sixteen waves a row 71; 301 rows 5.4 and 4.9)
+    else if (pieces <= 2048) SLIM_ROWS(2, 16);
+    else if (pieces <= 4096) SLIM_ROWS(4, 16);
+    else SLIM_ROWS(0, 16);
 #undef SLIM_ROWS
     SLIM_LAUNCH_CHECK();
     return SLIM_OK;
@@ -509,8 +513,10 @@ struct Tile {
 };
 template <int PLANES>
 struct Tiles {
-    static constexpr int count = 4;
-    static constexpr Tile list[4] = {{256, 256, 1, 7.0, 1.02, 1.60}, {128, 256, 1, 5.0, 0.60, 0.97}, {128, 128, 1, 4.3, 0.40, 0.55}, {64, 128, 2, 3.5, 0.28, 0.57}};
+    static constexpr int count = 5;
+    static constexpr Tile list[5] = {{256, 256, 1, 7.0, 1.02, 1.60}, {128, 256, 1, 5.0, 0.60, 0.97}, {128, 128, 1, 4.3, 0.40, 0.55},
+                                     {64, 128, 1, 3.3, 0.26, 0.28},      // four stages, a CU for each workgroup ...
+                                     {64, 128, 2, 3.5, 0.28, 0.57}};     // ... or three and two workgroups a CU
 };
 template <>
 struct Tiles<3> {                                        // (a wave's rows are a multiple of 48)
@@ -577,7 +583,7 @@ int launch_gemm8(const Gemm8Args& g, const Plan& p, hipStream_t st) {
 
 template <int PLANES>
 int gemm8(Gemm8Args g, void* slab, hipStream_t st) {
-    SLIM_PROF("gemm8", st, (double)g.rows * g.steps * 128 + (double)g.N * g.steps * 128 + (double)g.M * g.N * (g.dtype == SLIM_DTYPE_F32 ? 4 : 2),
+    SLIM_PROF("gemm8", st, (double)g.rows * g.steps * 128 + (double)g.N * g.steps * 128 + (double)g.M * g.N * element_size(g.dtype),
               2.0 * g.rows * g.N * g.steps * 128);
     const Plan p = plan_gemm8<PLANES>(g.rows, g.N, g.steps);
     g.tiles_m = (int)p.tiles_m, g.tiles_n = (int)p.tiles_n;
@@ -592,7 +598,8 @@ int gemm8(Gemm8Args g, void* slab, hipStream_t st) {
         else if (p.tile == 0) rc = launch_gemm8<PLANES, 0, 8, 4, 2, 4, 2, 2>(g, p, st);
         else if (p.tile == 1) rc = launch_gemm8<PLANES, 1, 4, 4, 2, 4, 3, 2>(g, p, st);
         else if (p.tile == 2) rc = launch_gemm8<PLANES, 2, 4, 2, 2, 4, 4, 2>(g, p, st);
-        else rc = launch_gemm8<PLANES, 3, 2, 2, 2, 4, 3, 4>(g, p, st);
+        else if (p.tile == 3) rc = launch_gemm8<PLANES, 3, 2, 2, 2, 4, 4, 2>(g, p, st);
+        else rc = launch_gemm8<PLANES, 4, 2, 2, 2, 4, 3, 4>(g, p, st);
     }
     if (rc || p.splits == 1) return rc;
     const int64_t threads = g.M * ((g.N + 3) / 4);
@@ -710,6 +717,7 @@ int launch_ring8_as(const RingArgs& g, hipStream_t st) {
 // against 20.3, but 64 x 5120 x 13824: 27.2 against 24.4).
 bool takes_ring(int64_t M, int64_t N) { return M <= 32 || (M <= 64 && N <= 8192); }
 int launch_ring8(const RingArgs& g, hipStream_t st) {
+    SLIM_PROF("ring8", st, (double)(g.N + g.M) * g.units * 128 + (double)g.M * g.N * element_size(g.dtype), 2.0 * g.M * g.N * g.units * 128);
     const bool narrow = g.N <= 4096;
     if (g.M <= 16) return narrow ? launch_ring8_as<1, 1, 8, 3>(g, st) : launch_ring8_as<1, 2, 4, 3>(g, st);
     if (g.M <= 32) return narrow ? launch_ring8_as<2, 1, 8, 2>(g, st) : launch_ring8_as<2, 2, 4, 2>(g, st);
@@ -851,6 +859,7 @@ __global__ __launch_bounds__(512) void token8_kernel(const TokenArgs g) {
 }
 template <typename T, int M, int NP>
 int launch_token8(const TokenArgs& g, int waves, hipStream_t st) {
+    SLIM_PROF("token8", st, (double)g.N * pad128(g.K) + (double)M * (g.N + g.K) * sizeof(T), 2.0 * M * g.N * g.K);
     const int bytes = 64 + M * (int)(ceil_div64(pad128(g.K), 1024) * 1024);
     // (two rows a wave and up to 768 workgroups, four rows and 512: 6.5 and 6.6 us at 4096 x 4096, 12.0 and 10.0 at 11008 x 4096)
     const int64_t pairs = ceil_div64(g.N, waves * 2), fours = ceil_div64(g.N, waves * 4);

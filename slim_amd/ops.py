@@ -1081,7 +1081,8 @@ def linear24_forward_q4(x, vals, meta, sf, N, bias, qL, qR, r, qblock, a_div, ws
 
 # ---- linears in 8-bit integers ------------------------------------------------------------------------------
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+# (None where torch is built without a GPU: the checks below refuse such tensors before these are needed)
+_raw_stream, _current_device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
 
 
 def _call_at(index, name, *args):
@@ -1371,6 +1372,8 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, beta1=0.9, bet
         sizes = [sizes[i] for i in keep]
         if not keep:
             return
+    if len(set(map(torch.Tensor.data_ptr, params))) < len(params):
+        raise ValueError("adamw_step: a parameter is in the list twice")
     lists = [x for x in (params, grads, ms, vs, ss, ws) if x is not None]
     words, at = _words(itertools.chain(*(map(torch.Tensor.data_ptr, x) for x in lists), sizes))       # one array after another
     starts = iter(range(at, at + words.itemsize * len(words), words.itemsize * len(params)))

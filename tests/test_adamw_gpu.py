@@ -287,6 +287,8 @@ def test_step_refusals(ops):
         kw = dict(masters=bad.get("masters"), norm=bad.get("norm"), scales=bad.get("scales"))
         with pytest.raises(ValueError):
             ops.adamw_step(bad["params"], bad["grads"], f, f, step=1, lr=0.1, **kw)
+    with pytest.raises(ValueError, match="twice"):
+        ops.adamw_step([p, p], [p, p], f * 2, f * 2, step=1, lr=0.1)
     with pytest.raises(TypeError):
         ops.adamw_step([p.double()], [p.double()], f, f, step=1, lr=0.1)
     with pytest.raises(ValueError):
