@@ -514,9 +514,9 @@ struct Tile {
 template <int PLANES>
 struct Tiles {
     static constexpr int count = 5;
-    static constexpr Tile list[5] = {{256, 256, 1, 7.0, 1.02, 1.60}, {128, 256, 1, 5.0, 0.60, 0.97}, {128, 128, 1, 4.3, 0.40, 0.55},
-                                     {64, 128, 1, 3.3, 0.26, 0.28},      // four stages, a CU for each workgroup ...
-                                     {64, 128, 2, 3.5, 0.28, 0.57}};     // ... or three and two workgroups a CU
+    static constexpr Tile list[5] = {{256, 256, 1, 7.0, 1.02, 1.60}, {128, 256, 1, 5.0, 0.60, 0.97}, {128, 128, 1, 4.3, 0.34, 0.53},
+                                     {64, 128, 1, 3.6, 0.24, 0.345},     // four stages, a CU for each workgroup ...
+                                     {64, 128, 2, 3.4, 0.34, 0.65}};     // ... or three and two workgroups a CU
 };
 template <>
 struct Tiles<3> {                                        // (a wave's rows are a multiple of 48)
