@@ -15,8 +15,10 @@ constexpr int NORM_CHUNK = 8192; // elements of a workgroup's step of the norm
 constexpr int NORM_TENSORS = 160;
 constexpr int STEP_TENSORS = 60;
 
-// a grid holds fewer than 2^32 threads; a tensor takes at most half of one
+// a grid holds fewer than 2^32 threads; a tensor takes at most half of one.  The norm's grid is NORM_BLOCKS whatever its tensors hold, so
+// a launch always takes NORM_TENSORS of them: its workspace, a partial sum per workgroup, is a function of their number alone.
 constexpr int64_t MAX_CHUNKS = (1 << 24) - 1, MAX_NUMEL = (int64_t)CHUNK << 23;
+static_assert(NORM_TENSORS * (MAX_NUMEL / NORM_CHUNK) < (int64_t)1 << 31, "the norm's chunks are counted in 32 bits");
 
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 
@@ -372,7 +374,7 @@ extern "C" int slim_grad_norm(const void* const* grads, const int64_t* numel, in
     for (int i = 0; i < count;) {
         NormArgs a;
         int64_t chunks = 0;
-        for (a.count = 0; a.count < NORM_TENSORS && i < count && chunks + norm_chunks_of(numel[i]) <= MAX_CHUNKS; ++a.count, ++i) {
+        for (a.count = 0; a.count < NORM_TENSORS && i < count; ++a.count, ++i) {
             a.g[a.count] = grads[i];
             a.n[a.count] = numel[i];
             a.first[a.count] = (uint32_t)chunks;

@@ -402,3 +402,11 @@ def test_optimizer_skips_and_refuses(ops):
         with torch.cuda.graph(graph):
             opt.step()
     copy.deepcopy(opt.state_dict())
+
+
+def test_norm_of_more_elements_than_a_grid_takes(ops):
+    """Nine times 2^34 elements: 18.9 million chunks of 8192, which a workgroup each would be more than a launch's 2^24."""
+    g = torch.zeros(2 ** 34, dtype=torch.bfloat16, device=DEV)
+    g[0], g[2 ** 33 + 12345], g[-1] = 3.0, 2.0, -5.0
+    norm = float(ops.grad_norm([g] * 9))
+    assert abs(norm - (9 * 38.0) ** 0.5) <= 2.0 ** -24 * (9 * 38.0) ** 0.5 * 1.01      # exact sums, a root in 64 bits, one rounding
