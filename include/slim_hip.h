@@ -554,7 +554,8 @@ int slim_transpose8(const int8_t* codes, int64_t N, int64_t K, int64_t ld, int8_
 int64_t slim_gemm8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int slim_gemm8_nt(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, const float* sb, int64_t M, int64_t N, int64_t K,
                   const void* bias, int dtype, void* out, int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream);
-/* y = the rows of x quantised as by slim_quantize_rows8, times the weight's codes [N, slim_rows8_ld(K)] as by slim_gemm8_nt. */
+/* y = the rows of x quantised as by slim_quantize_rows8, times the weight's codes [N, slim_rows8_ld(K)] as by slim_gemm8_nt.
+ * (A workspace of 0 bytes, here one or two rows of not too many channels, may be NULL.) */
 int64_t slim_linear8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int slim_linear8_forward(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, const int8_t* codes, const float* scale, int64_t N,
                          const void* bias, void* y, int64_t ldy, void* workspace, int64_t workspace_bytes, void* stream);
@@ -582,7 +583,8 @@ int64_t slim_adamw_blocks(int64_t numel);
  * up with probability equal to the value's place between its neighbours, with random bits that are a function of seed, the
  * tensor's ordinal first_index + i, and the position; a positive second moment never gets the code 0; a block that holds an
  * infinity or a NaN gets the scale NaN.
- * masters (16-bit parameters only) NULL: w is the parameter.  Otherwise w is masters[i] (fp32), and the parameter its rounding. */
+ * masters (16-bit parameters only) NULL: w is the parameter.  Otherwise w is masters[i] (fp32), and the parameter its rounding.
+ * eps: 0 (an element whose gradients have all been 0 then becomes NaN, as 0 / 0 is) or at least 2^-126.  Tensors do not overlap. */
 int slim_adamw_step(void* const* params, const void* const* grads, void* const* exp_avg, void* const* exp_avg_sq, float* const* scales,
                     float* const* masters, const int64_t* numel, int count, int dtype, int first_index, int64_t step, double lr, double beta1,
                     double beta2, double eps, double weight_decay, const float* norm, double max_norm, uint32_t seed, void* stream);

@@ -280,7 +280,9 @@ __device__ __forceinline__ void adamw_block(const StepArgs& a, int t, int64_t bl
             const float d = x[u][j] * clip;
             m[u][j] = m[u][j] * a.b1 + d * a.c1;
             v[u][j] = v[u][j] * a.b2 + (d * d) * a.c2;
-            const float denominator = __builtin_amdgcn_sqrtf(v[u][j]) * a.root + a.eps;
+            const bool low = v[u][j] < 0x1p-96f;         // (the instruction takes the root of a subnormal number for 0)
+            const float root = __builtin_amdgcn_sqrtf(low ? v[u][j] * 0x1p64f : v[u][j]) * (low ? 0x1p-32f : 1.f);
+            const float denominator = root * a.root + a.eps;
             w[u][j] = w[u][j] * a.keep - (m[u][j] * __builtin_amdgcn_rcpf(denominator)) * a.rate;
             if (EIGHT) {                                 // (elements behind the last were read as zeros and stay zeros)
                 top_m = max(top_m, f32_bits(m[u][j]) & 0x7fffffffu);
@@ -404,6 +406,7 @@ extern "C" int slim_adamw_step(void* const* params, const void* const* grads, vo
     SLIM_REQUIRE(known(dtype), "slim_adamw_step: unknown element type %d", dtype);
     SLIM_REQUIRE(step >= 1 && beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0 && lr >= 0 && weight_decay >= 0 && first_index >= 0,
                  "slim_adamw_step: step counts from 1, betas lie in [0, 1), lr, eps and weight_decay are not negative");
+    SLIM_REQUIRE(eps == 0 || eps >= 0x1p-126, "slim_adamw_step: eps is 0 or a normal fp32 number");
     SLIM_REQUIRE(!norm || max_norm > 0, "slim_adamw_step: max_norm must be positive");
     SLIM_REQUIRE(!masters || dtype != SLIM_DTYPE_F32, "slim_adamw_step: fp32 parameters need no master copies");
     const int64_t size = element_size(dtype);

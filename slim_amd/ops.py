@@ -1327,9 +1327,9 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, beta1=0.9, bet
 
     params, grads: lists of contiguous tensors of one element type (fp32, bf16, fp16).  Moments: fp32 tensors of the same sizes, or, with
     `scales` (fp32 [ceil(n / 512), 2] each), float8_e4m3fn first and float8_e5m2 second moments, rounded stochastically with
-    random bits that are a function of `seed`, the tensor's place first_index + i in the list and the position in it.  masters: fp32 copies
-    of 16-bit parameters, which are then their roundings.  norm (0-d fp32 tensor, grad_norm) with max_norm: the gradients are
-    multiplied by min(1, max_norm / (norm + 1e-6)) as they are read.  step counts from 1.  Empty tensors are left alone.  A captured call
+    random bits that are a function of `seed`, the tensor's place first_index + i in the list (empty tensors not counted) and the
+    position in it.  masters: fp32 copies of 16-bit parameters, which are then their roundings.  No two tensors that are updated overlap.  norm (0-d fp32 tensor, grad_norm) with max_norm: the gradients are
+    multiplied by min(1, max_norm / (norm + 1e-6)) as they are read.  step counts from 1; eps is 0 or at least 2^-126.  Empty tensors are left alone.  A captured call
     replays with the step, lr and seed that it was captured with."""
     params, grads, ms, vs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
     ss, ws = None if scales is None else list(scales), None if masters is None else list(masters)
@@ -1372,12 +1372,13 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, beta1=0.9, bet
         sizes = [sizes[i] for i in keep]
         if not keep:
             return
-    if len(set(map(torch.Tensor.data_ptr, params))) < len(params):
-        raise ValueError("adamw_step: a parameter is in the list twice")
-    lists = [x for x in (params, grads, ms, vs, ss, ws) if x is not None]
-    words, at = _words(itertools.chain(*(map(torch.Tensor.data_ptr, x) for x in lists), sizes))       # one array after another
+    lists = [x for x in (grads, params, ms, vs, ss, ws) if x is not None]
+    addresses = [a for x in lists for a in map(torch.Tensor.data_ptr, x)]
+    if len(set(addresses[len(grads):])) < len(addresses) - len(grads):
+        raise ValueError("adamw_step: a tensor that is updated is in the lists twice")
+    words, at = _words(itertools.chain(addresses, sizes))                # one array after another
     starts = iter(range(at, at + words.itemsize * len(words), words.itemsize * len(params)))
-    arrays = [None if x is None else next(starts) for x in (params, grads, ms, vs, ss, ws)] + [next(starts)]
-    _call_at(gpu, "slim_adamw_step", *arrays, len(params), dt, int(first_index), int(step), float(lr), float(beta1), float(beta2), float(eps),
+    arrays = [None if x is None else next(starts) for x in (grads, params, ms, vs, ss, ws)] + [next(starts)]
+    _call_at(gpu, "slim_adamw_step", arrays[1], arrays[0], *arrays[2:], len(params), dt, int(first_index), int(step), float(lr), float(beta1), float(beta2), float(eps),
              float(weight_decay), _p(norm), 0.0 if max_norm is None else float(max_norm), int(seed) & 0xffffffff)
-    torch.autograd.graph.increment_version(params)
+    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])

@@ -27,6 +27,8 @@ class AdamW(torch.optim.Optimizer):
                  max_grad_norm=None, seed=0):
         if not lr >= 0 or not eps >= 0 or not weight_decay >= 0:
             raise ValueError(f"lr, eps and weight_decay must not be negative, got {lr}, {eps}, {weight_decay}")
+        if 0 < eps < 2.0 ** -126:
+            raise ValueError(f"eps must be 0 or at least 2^-126, got {eps}")
         if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
             raise ValueError(f"betas must lie in [0, 1), got {betas}")
         if state_bits not in (8, 32):
@@ -93,8 +95,7 @@ class AdamW(torch.optim.Optimizer):
             state = self.state[p]
             if not state:
                 state.update(self._new_state(p, group))
-            state["step"] += 1
-            key = (id(group), p.dtype, "scales" in state, "master" in state, state["step"])
+            key = (id(group), p.dtype, "scales" in state, "master" in state, state["step"] + 1)
             calls.setdefault(key, (group, []))[1].append((p, g, state))
         first = 0
         for (_, _, eight, master, step), (group, members) in calls.items():
@@ -105,11 +106,22 @@ class AdamW(torch.optim.Optimizer):
                            masters=[s["master"] for s in states] if master else None, seed=self.seed + step * 0x9e3779b1, norm=norm,
                            max_norm=self.max_grad_norm, first_index=first)
             first += len(members)
+            for state in states:
+                state["step"] = step
         return loss
 
+    def __getstate__(self):
+        return dict(super().__getstate__(), max_grad_norm=self.max_grad_norm, seed=self.seed, last_norm=self.last_norm)
+
     def load_state_dict(self, state_dict):
-        """torch's, with the state's own element types (which it would change to the parameters')."""
+        """torch's, with the state's own element types (which it would change to the parameters').  What torch.optim.AdamW saved over
+        fp32 parameters loads too (its moments continue in 32 bits)."""
         super().load_state_dict(state_dict)
+        for group in self.param_groups:
+            for name in ("state_bits", "master_weights"):
+                group.setdefault(name, self.defaults[name])
+        for state in self.state.values():
+            state["step"] = int(state["step"])
         ids = [i for group in state_dict["param_groups"] for i in group["params"]]
         params = [p for group in self.param_groups for p in group["params"]]
         for i, p in zip(ids, params):

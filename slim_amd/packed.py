@@ -270,7 +270,7 @@ class Int8Linear(torch.nn.Module):
     def forward(self, x):
         if x.shape[-1] != self.in_features:
             raise ValueError(f"Int8Linear: the input has {x.shape[-1]} channels, the weight {self.in_features}")
-        if torch.is_autocast_enabled("cuda") and x.dtype == torch.float32:
+        if torch.is_autocast_enabled("cuda") and x.dtype in (torch.float32, torch.bfloat16, torch.float16):
             x = x.to(torch.get_autocast_dtype("cuda"))
         x2 = x.reshape(-1, self.in_features)
         y = _Int8Product.apply(x2, self) if torch.is_grad_enabled() and x2.requires_grad else self.product(x2)

@@ -410,3 +410,70 @@ def test_norm_of_more_elements_than_a_grid_takes(ops):
     g[0], g[2 ** 33 + 12345], g[-1] = 3.0, 2.0, -5.0
     norm = float(ops.grad_norm([g] * 9))
     assert abs(norm - (9 * 38.0) ** 0.5) <= 2.0 ** -24 * (9 * 38.0) ** 0.5 * 1.01      # exact sums, a root in 64 bits, one rounding
+
+
+def test_second_moments_below_the_normal_range(ops):
+    """eps = 0: what a step does depends on the ratio of the moments alone, down to gradients whose squares are subnormal."""
+    n = 517
+    gen = torch.Generator().manual_seed(5)
+    g0 = (torch.rand(n, generator=gen) * 9 + 1) * 1e-19 * torch.randint(0, 2, (n,), generator=gen).mul(2).sub(1)
+    zero = torch.zeros(n)
+    p, g, m, v = to_dev([zero], [g0], [zero], [zero])
+    ops.adamw_step(p, g, m, v, step=1, lr=1e-2, eps=0.0)
+    ew, _, ev, update = formula(zero, g0, zero, zero, 1, eps=0.0, weight_decay=0.0)
+    assert float(ev.max()) < 2.0 ** -126
+    # the square and its product with 1 - beta2 are each rounded to a multiple of 2^-149: half of that twice, and half its
+    # relative size in the root; the rest as in the normal range
+    rounding = 2.0 ** -149 / ev.double()
+    assert bool(((p[0].cpu().double() - ew).abs() <= update.abs() * (0.5 * rounding * 1.01 + 17 * 2.0 ** -24)).all())
+
+
+def test_step_refuses_shared_state_and_takes_inference_tensors(ops):
+    p, q, m, v, s = (torch.zeros(8, device=DEV) for _ in range(5))
+    for lists in (([p, q], [m, m], [v, s]), ([p], [m], [m]), ([p], [p], [v])):
+        with pytest.raises(ValueError, match="twice"):
+            ops.adamw_step(lists[0], lists[0], lists[1], lists[2], step=1, lr=0.1)
+    with pytest.raises(ValueError, match="eps"):
+        ops.adamw_step([p], [q], [m], [v], step=1, lr=0.1, eps=2.0 ** -127)
+    with torch.inference_mode():
+        w = torch.ones(8, device=DEV)
+        ops.adamw_step([w, p], [torch.ones(8, device=DEV)] * 2, [m, q], [v, s], step=1, lr=0.1, weight_decay=0.0)
+    assert bool((w < 0.91).all()) and bool((p < -0.09).all())
+    with torch.no_grad():
+        g = torch.ones(8, device=DEV)
+        ops.adamw_step([g], [g], [torch.zeros(8, device=DEV)], [torch.zeros(8, device=DEV)], step=1, lr=0.1)     # its own gradient: read first
+    assert bool(((g - 0.9).abs() < 1e-6).all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_optimizer_copies(ops, bits):
+    """A deep copy goes on exactly as the original does; gradients that are refused leave the step count alone."""
+    from slim_amd.optim import AdamW
+    a = small_model(torch.float32)
+    opt = AdamW(a.parameters(), lr=1e-2, state_bits=bits, max_grad_norm=1.0, seed=3)
+    run_steps(a, opt, 3)
+    b, twin = copy.deepcopy((a, opt))
+    run_steps(a, opt, 3, seed=7)
+    run_steps(b, twin, 3, seed=7)
+    assert all(torch.equal(x, y) for x, y in zip(a.parameters(), b.parameters())) and torch.equal(opt.last_norm, twin.last_norm)
+    p = next(a.parameters())
+    opt.state[p]["exp_avg"] = opt.state[p]["exp_avg"][:1]
+    with pytest.raises(ValueError):
+        opt.step()
+    assert opt.state[p]["step"] == 6
+
+
+def test_optimizer_continues_from_torchs_state(ops):
+    from slim_amd.optim import AdamW
+    a, b = small_model(torch.float32), small_model(torch.float32)
+    x, y = torch.optim.AdamW(a.parameters(), lr=1e-2), torch.optim.AdamW(b.parameters(), lr=1e-2)
+    run_steps(a, x, 5)
+    run_steps(b, y, 5)
+    z = AdamW(b.parameters(), lr=1e-3)
+    z.load_state_dict(copy.deepcopy(y.state_dict()))
+    run_steps(a, x, 5, seed=2)
+    run_steps(b, z, 5, seed=2)
+    for p, q in zip(a.parameters(), b.parameters()):
+        # five updates of relative error 40 * 2^-24 on either side, each below lr * 10, and the sums' roundings
+        assert bool(((p - q).abs() <= 5 * 2 * (40 * 2.0 ** -24 * 0.1 + 4 * 2.0 ** -24 * (p.abs() + 0.1))).all())
+        assert z.state[q]["step"] == 10

@@ -194,3 +194,18 @@ def test_files_of_the_other_kind_are_refused(gpu, tmp_path):
     model.model.layers = torch.nn.ModuleList([Block()])
     with pytest.raises(ValueError, match="no PackedLinear or Int8Linear"):
         save_packed(model, str(tmp_path / "x"))
+
+
+def test_autocast_decides_the_type(gpu):
+    """As for nn.Linear: under autocast the input of any 16- or 32-bit type is taken in autocast's type."""
+    from slim_amd.packed import Int8Linear
+    lin, _ = compressed_linear(100, 300)
+    del lin.lora_left, lin.lora_right
+    lin._forward_hooks.clear()
+    m = Int8Linear(lin)
+    x = torch.randn(5, 300, device=DEV)
+    for to in (torch.bfloat16, torch.float16):
+        for dtype in (torch.float32, torch.bfloat16, torch.float16):
+            with torch.autocast("cuda", dtype=to):
+                y = m(x.to(dtype))
+            assert y.dtype == to and torch.equal(y, m(x.to(dtype).to(to)))
