@@ -336,3 +336,63 @@ def test_padded_c_abi_rows_of_codes(ops):
     _lib.call("slim_quantize_rows8", x.data_ptr(), 0, 9, 150, 150, codes.data_ptr(), 400, scale.data_ptr(), torch.cuda.current_stream().cuda_stream)
     want, _ = definition(x)
     assert torch.equal(codes[:, :150].cpu(), want) and not bool(codes[:, 150:256].any()) and bool((codes[:, 256:] == 9).all())
+
+
+# 128 x 256, 64 x 128 with two workgroups a CU, and 128 x 128 and 64 x 128 in slices
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(1030, 5000, 300), (600, 9001, 300), (301, 9001, 300), (128, 5121, 13700), (130, 5121, 9000), (500, 2003, 9000)])
+def test_more_tiles_against_64_bits(ops, M, N, K, dtype):
+    test_large_products_against_64_bits(ops, M, N, K, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(300, 600, 5000), (301, 2000, 5001), (129, 9001, 1000), (257, 9001, 1100), (600, 1000, 5003)])
+def test_more_gradient_tiles_against_64_bits(ops, M, N, K, dtype):
+    test_large_gradients_against_64_bits(ops, M, N, K, dtype)
+
+
+def sampled_rows_equal(ops, y, x, codes, scale, bias, rows):
+    """Rows of a product against the exact sums of their codes: the fp32 operations of the definition, so bit for bit."""
+    xc, xs = ops.quantize_rows8(x[rows])
+    sums = torch.stack([(c[None, :].double() * codes.double()).sum(1) for c in xc]) if codes.numel() < 1 << 24 else torch.cat(
+        [torch.stack([(c[None, :].double() * part.double()).sum(1) for c in xc]) for part in codes.split(1 << 10)], 1)
+    want = sums.float() * xs[:, None] * scale
+    want = (want if bias is None else want + bias.float()).to(y.dtype)
+    return same(y[rows], want)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 8191, 14336), (1, 8192, 14337), (1, 300, 28672), (1, 300, 28673), (2, 8191, 8192), (2, 8193, 8193), (2, 300, 16384), (2, 300, 16385),
+                                   (3, 4096, 1000), (16, 4097, 1000), (17, 4096, 1000), (32, 4097, 1000), (33, 4096, 1000), (33, 4097, 1000), (64, 8192, 500), (64, 8193, 500),
+                                   (65, 8192, 500), (5, 260, 131071)])
+def test_borders_of_the_kernels_for_few_tokens(ops, M, N, K):
+    x = torch.randn(M, K, device=DEV).bfloat16()
+    codes, scale = ops.quantize_rows8(torch.randn(N, K, device=DEV))
+    bias = torch.randn(N, device=DEV).bfloat16()
+    y = ops.linear8_forward(x, codes, scale, bias)
+    assert sampled_rows_equal(ops, y, x, codes, scale, bias, list(range(M)) if M < 4 else [0, M // 2, M - 1])
+
+
+def test_offsets_beyond_32_bits(ops):
+    """A result, rows of a 16-bit input, and a weight's codes of more than 2^31 elements each; the last rows, where an offset counts."""
+    codes, scale = ops.quantize_rows8(torch.randn(32000, 64, device=DEV))
+    x = torch.randn(70001, 64, device=DEV).bfloat16()
+    y = ops.linear8_forward(x, codes, scale)
+    assert y.numel() > 2 ** 31 and sampled_rows_equal(ops, y, x, codes, scale, None, [0, 67108, 67109, 69999, 70000])
+    del y, x
+    x = torch.randn(300001, 8192, device=DEV, dtype=torch.bfloat16)
+    c, s = ops.quantize_rows8(x)
+    want, want_scale = definition(x[-3:])
+    assert torch.equal(c[-3:].cpu(), want) and same(s[-3:].cpu(), want_scale)
+    del x, c, s
+    N, K = 17001, 131071
+    codes = torch.randint(-127, 128, (N, pad(K)), dtype=torch.int8, device=DEV)
+    codes[:, K:] = 0
+    scale = torch.rand(N, device=DEV)
+    assert codes.numel() > 2 ** 31
+    for M in (1, 5, 70):
+        x = torch.randn(M, K, device=DEV).bfloat16()
+        y = ops.linear8_forward(x, codes, scale)
+        assert sampled_rows_equal(ops, y[:, -600:], x, codes[-600:], scale[-600:], None, [0, M - 1])
+        assert sampled_rows_equal(ops, y[:, :600], x, codes[:600], scale[:600], None, [0, M - 1])
+    t = ops.transpose8(codes[:, :128 * 7].contiguous(), 128 * 7 - 5)
+    assert torch.equal(t[:, :N], codes[:, :128 * 7 - 5].t()) and not bool(t[:, N:].any())
