@@ -288,6 +288,54 @@ __device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int spl
     tn = r / gm;
 }
 
+// The runs of consecutive columns that a lane holds of a row of its wave's part, 4 FN values: eight per two fragments, four of an odd last one.
+// each(n0, fq, take) calls take(how many, first value, column) for each.
+template <int FN>
+struct Columns {
+    static constexpr int PAIRS = FN / 2 * 32, RUNS = (FN + 1) / 2;
+    template <typename F>
+    static __device__ __forceinline__ void each(int64_t n0, int fq, F take) {
+#pragma unroll
+        for (int c = 0; c < FN / 2; ++c) take(std::integral_constant<int, 8>(), c * 8, n0 + c * 32 + fq * 8);
+        if constexpr (FN % 2) take(std::integral_constant<int, 4>(), 4 * FN - 4, n0 + PAIRS + fq * 4);
+    }
+};
+
+// A wave's sums, planes joined, scaled, with the bias, rounded and stored: rows 16 (group0 + i) + fr of the result.
+template <int PLANES, int FM, int FN>
+__device__ __forceinline__ void write_results(const Gemm8Args& g, const i32x4 (&acc)[FM][FN], const float (&sa)[FM / PLANES], const float (&sb)[4 * FN],
+                                              int64_t group0, int64_t n0, int fr, int fq) {
+    float bias[4 * FN];
+#pragma unroll
+    for (int c = 0; c < 4 * FN; ++c) bias[c] = 0.f;
+    if (g.bias) {
+        auto load = [&](const auto* p) { Columns<FN>::each(n0, fq, [&](auto count, int c, int64_t n) { load_run<count.value>(p + n, g.N - n, bias + c); }); };
+        if (g.dtype == SLIM_DTYPE_F32) load((const float*)g.bias);
+        else if (g.dtype == SLIM_DTYPE_BF16) load((const bf16_t*)g.bias);
+        else load((const _Float16*)g.bias);
+#pragma unroll
+        for (int c = 0; c < 4 * FN; ++c) asm volatile("" : "+v"(bias[c]));     // (arrived: no wait for them is left to whoever follows)
+    }
+    auto rows = [&](auto* out, auto convert) {
+#pragma unroll
+        for (int i = 0; i < FM / PLANES; ++i) {
+            const int64_t m = (group0 + i) * 16 + fr;
+            if (m >= g.M) continue;
+            auto value = [&](int c) {
+                int sums[PLANES];
+#pragma unroll
+                for (int p = 0; p < PLANES; ++p) sums[p] = acc[i * PLANES + p][c >> 2][c & 3];
+                const float v = (join_planes<PLANES>(sums, 1) * sa[i]) * sb[c];
+                return convert(g.bias ? v + bias[c] : v);
+            };
+            Columns<FN>::each(n0, fq, [&](auto count, int c, int64_t n) { store_run<count.value>(out + m * g.ldo + n, g.N - n, [&](int k) { return value(c + k); }); });
+        }
+    };
+    if (g.dtype == SLIM_DTYPE_F32) rows((float*)g.out, [](float v) { return v; });
+    else if (g.dtype == SLIM_DTYPE_BF16) rows((bf16_t*)g.out, [](float v) { return f32_to_bf16(v); });
+    else rows((_Float16*)g.out, [](float v) { return (_Float16)v; });
+}
+
 // D = A B^T on 16 x 16 x 64 int8 instructions, operands delivered by LDS-DMA (16 bytes per lane) a 128-byte step ahead, two
 // stages.  LDS image of a stage: BM rows of A, then BN rows of B, 128 bytes each; the 16-byte piece c of a row is stored at
 // c ^ key(row), applied on the source side.  The result is computed transposed (B's fragment as the first operand): a lane then holds
@@ -421,58 +469,193 @@ __device__ __forceinline__ void gemm8_tile(const Gemm8Args& g, char* lds, int64_
     }
     // everything the epilogue reads is requested at once (loaded row by row it costs a trip to memory per row: 4 us of a 256 x 256 tile)
     const int64_t group0 = (row0 / 16 + wr * FM) / PLANES;
-    float sa[FM / PLANES], sb[4 * FN], bias[4 * FN];
+    float sa[FM / PLANES], sb[4 * FN];
 #pragma unroll
     for (int i = 0; i < FM / PLANES; ++i) sa[i] = g.sa[min((group0 + i) * 16 + fr, g.M - 1)];
 #pragma unroll
-    for (int c = 0; c < 4 * FN; ++c) sb[c] = 1.f, bias[c] = 0.f;
-    auto columns = [&](auto take) {                      // take(first value, how many, column) for each of the lane's runs of columns
-#pragma unroll
-        for (int c = 0; c < FN / 2; ++c) take(std::integral_constant<int, 8>(), c * 8, n0 + c * 32 + fq * 8);
-        if constexpr (FN % 2) take(std::integral_constant<int, 4>(), 4 * FN - 4, n0 + PAIRS + fq * 4);
-    };
-    if (g.sb) columns([&](auto count, int c, int64_t n) { load_run<count.value>(g.sb + n, g.N - n, sb + c); });
-    if (g.bias) {
-        if (g.dtype == SLIM_DTYPE_F32) columns([&](auto count, int c, int64_t n) { load_run<count.value>((const float*)g.bias + n, g.N - n, bias + c); });
-        else if (g.dtype == SLIM_DTYPE_BF16) columns([&](auto count, int c, int64_t n) { load_run<count.value>((const bf16_t*)g.bias + n, g.N - n, bias + c); });
-        else columns([&](auto count, int c, int64_t n) { load_run<count.value>((const _Float16*)g.bias + n, g.N - n, bias + c); });
-    }
-    auto rows = [&](auto* out, auto convert) {
-#pragma unroll
-        for (int i = 0; i < FM / PLANES; ++i) {
-            const int64_t m = (group0 + i) * 16 + fr;
-            if (m >= g.M) continue;
-            auto value = [&](int c) {
-                int sums[PLANES];
-#pragma unroll
-                for (int p = 0; p < PLANES; ++p) sums[p] = acc[i * PLANES + p][c >> 2][c & 3];
-                const float v = (join_planes<PLANES>(sums, 1) * sa[i]) * sb[c];
-                return convert(g.bias ? v + bias[c] : v);
-            };
-            columns([&](auto count, int c, int64_t n) { store_run<count.value>(out + m * g.ldo + n, g.N - n, [&](int k) { return value(c + k); }); });
-        }
-    };
-    if (g.dtype == SLIM_DTYPE_F32) rows((float*)g.out, [](float v) { return v; });
-    else if (g.dtype == SLIM_DTYPE_BF16) rows((bf16_t*)g.out, [](float v) { return f32_to_bf16(v); });
-    else rows((_Float16*)g.out, [](float v) { return (_Float16)v; });
+    for (int c = 0; c < 4 * FN; ++c) sb[c] = 1.f;
+    if (g.sb) Columns<FN>::each(n0, fq, [&](auto count, int c, int64_t n) { load_run<count.value>(g.sb + n, g.N - n, sb + c); });
+    write_results<PLANES, FM, FN>(g, acc, sa, sb, group0, n0, fr, fq);
 }
 
-// REST > 0: behind the columns of full tiles lie g.rest_n columns of tiles of 16 REST WN columns (the last round of workgroups).
-template <int PLANES, int FM, int FN, int WM, int WN, int STAGES, int OCC, int REST>
+template <int PLANES, int FM, int FN, int WM, int WN, int STAGES, int OCC>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm8_kernel(const Gemm8Args g) {
-    constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     int tm, tn, slice;
-    if constexpr (REST > 0) {
-        const int full = g.tiles_m * g.tiles_n;
-        if ((int)blockIdx.x >= full) {
-            tile_of((int)blockIdx.x - full, g.tiles_m, g.rest_n, 1, tm, tn, slice);
-            gemm8_tile<PLANES, FM, REST, WM, WN, STAGES>(g, lds, (int64_t)tm * BM, (int64_t)g.tiles_n * BN + (int64_t)tn * 16 * REST * WN, 0);
-            return;
-        }
-    }
     tile_of(blockIdx.x, g.tiles_m, g.tiles_n, g.splits, tm, tn, slice);
-    gemm8_tile<PLANES, FM, FN, WM, WN, STAGES>(g, lds, (int64_t)tm * BM, (int64_t)tn * BN, slice);
+    gemm8_tile<PLANES, FM, FN, WM, WN, STAGES>(g, lds, (int64_t)tm * 16 * FM * WM, (int64_t)tn * 16 * FN * WN, slice);
+}
+
+// The same product by workgroups that stay, for more tiles than CUs: each takes every gridDim.x-th tile, and the stream of requests
+// runs on from one tile into the next, so that the next tile's first steps travel while the finished one is scaled and stored, and its
+// stores drain under the next tile's products (a workgroup a tile: 4096 x 11008 x 4096 164 us, 159 so; 8192^3 399 and 382, 8192 x 4096 x
+// 1024 47 and 41).  REST > 0: behind the columns of full tiles lie g.rest_n columns of tiles of 16 REST WN columns, which fill the last
+// round of workgroups better.  The scales of a tile come by LDS-DMA while it is multiplied.  (g.steps >= 2)
+template <int PLANES, int FM, int FN, int WM, int WN, int REST>
+__global__ __launch_bounds__(64 * WM * WN, 2) void gemm8_stream_kernel(const Gemm8Args g) {
+    constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN, NW = WM * WN, STAGE_BYTES = (BM + BN) * 128;
+    constexpr int ALOADS = BM / 8 / NW, LOADS = (BM + BN) / 8 / NW;      // requests of a wave and step: eight rows each, A's first
+    static_assert(BM % 64 == 0 && BM % (8 * NW) == 0 && 16 * WN % (8 * NW) == 0 && BM + BN <= 64 * NW, "requests and scales are dealt out evenly");
+    constexpr int LEAST = REST && REST < FN ? REST : FN, STORES = FM / PLANES * Columns<LEAST>::RUNS, STORES32 = FM / PLANES * LEAST;     // of a whole tile, at least
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    float* const scales = (float*)(lds + 2 * STAGE_BYTES);              // [BM] of the rows, [BN] of the columns
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wave / WN, wc = wave % WN, fr = lane & 15, fq = lane >> 4;
+    const int full = g.tiles_m * g.tiles_n, total = full + g.tiles_m * g.rest_n, steps = g.steps;
+    // what depends on the lane and is needed once a tile is computed anew, not kept over the loop, where 250 of 256 registers are taken
+    auto this_lane = []() {
+        uint32_t zero = 0;
+        asm volatile("" : "+v"(zero));
+        return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, zero));
+    };
+    auto place = [&](int b, int64_t& row0, int64_t& col0) {
+        int tm, tn, slice;
+        if (REST && b >= full) {
+            tile_of(b - full, g.tiles_m, g.rest_n, 1, tm, tn, slice);
+            col0 = (int64_t)g.tiles_n * BN + (int64_t)tn * 16 * REST * WN;
+        } else {
+            tile_of(b, g.tiles_m, g.tiles_n, 1, tm, tn, slice);
+            col0 = (int64_t)tn * BN;
+        }
+        row0 = (int64_t)tm * BM;
+    };
+    // where the requests are: tile, step, this lane's sources in it (as in gemm8_tile; in a narrow tile the rows behind its own are never read)
+    int at = blockIdx.x, ks = 0;
+    const int8_t *pa, *pb;
+    uint32_t off[LOADS];
+    auto aim = [&]() {
+        int64_t row0, col0;
+        place(at, row0, col0);
+        pa = g.A + row0 * g.lda, pb = g.B + col0 * g.ldb;
+        const bool narrow = REST && at >= full;
+        const int l = this_lane(), pr = l >> 3, pc = l & 7;
+#pragma unroll
+        for (int s = 0; s < LOADS; ++s) {
+            const int R = (s * NW + wave) * 8 + pr;
+            if (s < ALOADS) {
+                off[s] = (uint32_t)(min((int64_t)R, g.rows - 1 - row0) * g.lda) + (pc ^ (R & 7)) * 16;
+            } else {
+                const int r = R - BM, w = narrow ? r % (16 * (REST ? REST : 1)) : r % (16 * FN), pairs = narrow ? Columns<REST>::PAIRS : Columns<FN>::PAIRS;
+                const int key = w < pairs ? (w & 3) | (((w >> 3) & 1) << 2) : w & 7;
+                off[s] = (uint32_t)(min((int64_t)r, g.N - 1 - col0) * g.ldb) + (pc ^ key) * 16;
+            }
+        }
+    };
+    auto advance = [&]() {                               // (behind the last tile: its last step again, which nothing reads)
+        if (at + (int)gridDim.x < total) at += gridDim.x, ks = 0, aim();
+        else ks = steps - 1;
+    };
+    auto request = [&](auto loads, int stage) {
+        const int64_t k = (int64_t)ks * 128;
+#pragma unroll
+        for (int s = 0; s < loads.value; ++s)
+            __builtin_amdgcn_global_load_lds((glb_ptr_t)((s < ALOADS ? pa : pb) + k + off[s]), (lds_ptr_t)(lds + stage * STAGE_BYTES + (s * NW + wave) * 1024), 16, 0, 0);
+        ++ks;
+    };
+    aim();
+    request(std::integral_constant<int, LOADS>(), 0);
+    request(std::integral_constant<int, LOADS>(), 1);    // (steps >= 2)
+    wait_vmcnt<LOADS>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+
+    int b = blockIdx.x, stage = 0;
+    bool stores = false;                                 // the tile before stored all of its rows and columns
+    auto tiles = [&](auto width, int end) {              // this workgroup's tiles in front of `end`, all `width` fragments wide
+        constexpr int F = width.value, PAIRS = Columns<F>::PAIRS, L = ALOADS + (LOADS - ALOADS) * F / FN;
+        constexpr int READS = FM + F, PRODUCTS = FM * F, PACE1 = PRODUCTS / READS, PACE2 = PRODUCTS / (READS + L);
+        if (b >= end) return;
+        const int x0 = (fq ^ (fr & 7)) * 16;
+        const int a_off = (wr * 16 * FM + fr) * 128 + x0;
+        const int b_off = (BM + wc * 16 * F + (fr >> 2) * 8 + (fr & 3)) * 128 + x0;
+        const int odd_off = (BM + wc * 16 * F + PAIRS + fr) * 128 + x0;
+        i32x4 af[2][FM], bf[2][F];
+        auto read = [&](int half, int st) {
+            const char* pa = lds + ((st * STAGE_BYTES + a_off) ^ (half * 64));
+            const char* pb = lds + ((st * STAGE_BYTES + b_off) ^ (half * 64));
+#pragma unroll
+            for (int j = 0; j < F / 2 * 2; ++j) bf[half][j] = *(const i32x4*)(pb + ((j >> 1) * 32 + (j & 1) * 4) * 128);
+            if (F % 2) bf[half][F - 1] = *(const i32x4*)(lds + ((st * STAGE_BYTES + odd_off) ^ (half * 64)));
+#pragma unroll
+            for (int i = 0; i < FM; ++i) af[half][i] = *(const i32x4*)(pa + i * 16 * 128);
+        };
+        for (; b < end; b += gridDim.x) {
+            int64_t row0, col0;
+            place(b, row0, col0);
+            read(0, stage);                              // (again: kept over the end of the tile before they would not fit the registers)
+            i32x4 acc[FM][F];
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < F; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+            auto multiply = [&](int half) {
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int j = 0; j < F; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bf[half][j], af[half][i], acc[i][j], 0, 0, 0);
+            };
+            for (int kt = 0; kt < steps; ++kt) {
+                if (ks >= steps) advance();
+                __builtin_amdgcn_sched_barrier(0);
+                read(1, stage);
+                multiply(0);
+#pragma unroll
+                for (int s = 0; s < READS; ++s) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, PACE1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                // this wave's reads of the stage are done and its requests of the next one have landed (at a tile's first step they
+                // are older than the stores of the tile before, which need not be waited for); behind the barrier so are everyone's
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                if (kt || !stores) wait_vmcnt<0>();
+                else if (g.dtype == SLIM_DTYPE_F32) wait_vmcnt<STORES32>();
+                else wait_vmcnt<STORES>();
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                if (kt == 0) {                           // every wave is past the tile before: this one's scales, for its end
+                    const int t = wave * 64 + this_lane();
+                    const float* src = wave * 64 < BM ? g.sa + min(row0 / PLANES + t, g.M - 1) : g.sb + min(col0 + t - BM, g.N - 1);
+                    if (wave * 64 < BM || (g.sb && wave * 64 < BM + BN)) __builtin_amdgcn_global_load_lds((glb_ptr_t)src, (lds_ptr_t)(scales + wave * 64), 4, 0, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                read(0, stage ^ 1);
+                request(std::integral_constant<int, L>(), stage);
+                multiply(1);
+#pragma unroll
+                for (int s = 0; s < READS; ++s) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, PACE2, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                }
+#pragma unroll
+                for (int s = 0; s < L; ++s) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, PACE2, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                stage ^= 1;
+            }
+            asm volatile("" ::: "memory");               // (no store moves in front of the requests)
+            const int l = this_lane(), er = l & 15, eq = l >> 4;
+            float sa[FM / PLANES], sb[4 * F];
+#pragma unroll
+            for (int i = 0; i < FM / PLANES; ++i) sa[i] = scales[(wr * FM / PLANES + i) * 16 + er];
+#pragma unroll
+            for (int c = 0; c < 4 * F; ++c) sb[c] = 1.f;
+            const int64_t n0 = col0 + wc * 16 * F;
+            if (g.sb)
+                Columns<F>::each(n0, eq, [&](auto count, int c, int64_t n) {
+#pragma unroll
+                    for (int j = 0; j < count.value; ++j) sb[c + j] = scales[BM + (int)(n - col0) + j];
+                });
+            write_results<PLANES, FM, F>(g, acc, sa, sb, (row0 / 16 + wr * FM) / PLANES, n0, er, eq);
+            asm volatile("" ::: "memory");
+            stores = row0 / PLANES + BM / PLANES <= g.M && col0 + 16 * F * WN <= g.N;
+        }
+    };
+    tiles(std::integral_constant<int, FN>(), full);
+    if constexpr (REST > 0) tiles(std::integral_constant<int, REST>(), total);
+    wait_vmcnt<0>();                                     // (the requests behind the last step land before the LDS is given up)
 }
 
 // The slices' sums added (whole numbers: any order gives the same), planes joined, scaled and rounded: a thread per four columns.
@@ -528,6 +711,7 @@ struct Plan {
     int64_t tiles_m = 0, tiles_n = 0, slab_rows = 0, slab_cols = 0;
     int rest = 0;                                        // fragments (of 64 columns) of the narrower tiles behind the full ones
     int64_t rest_n = 0;
+    bool stays() const { return tile == 0 && splits == 1 && steps_per_split >= 2 && tiles_m * (tiles_n + rest_n) > 256; }     // workgroups take several tiles
     int64_t slab_bytes() const { return splits > 1 ? splits * slab_rows * slab_cols * 4 : 0; }
 };
 template <int PLANES>
@@ -555,7 +739,7 @@ Plan plan_gemm8(int64_t rows, int64_t N, int64_t steps) {
     }
     // The largest tile's last round, when it is not full, on narrower tiles that fill it better (4096 x 11008: 512 full tiles and 240 of
     // 192 columns in place of 176 full ones).
-    if (PLANES < 3 && best.tile == 0 && best.splits == 1 && best.tiles_m <= 256) {
+    if (PLANES < 3 && best.tile == 0 && best.splits == 1 && best.steps_per_split >= 2 && best.tiles_m <= 256) {
         const int64_t tiles = best.tiles_m * best.tiles_n, columns = tiles / 256 * 256 / best.tiles_m;
         if (tiles > 256 && tiles % 256 && columns < best.tiles_n) {
             for (int rest = 3; rest >= 2; --rest) {
@@ -568,15 +752,27 @@ Plan plan_gemm8(int64_t rows, int64_t N, int64_t steps) {
     return best;
 }
 
-template <int PLANES, int TILE, int FM, int FN, int WM, int WN, int STAGES, int OCC, int REST = 0>
+template <int PLANES, int TILE, int FM, int FN, int WM, int WN, int STAGES, int OCC>
 int launch_gemm8(const Gemm8Args& g, const Plan& p, hipStream_t st) {
     constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN, bytes = STAGES * (BM + BN) * 128;
-    const int64_t blocks = p.tiles_m * p.tiles_n * p.splits + p.tiles_m * p.rest_n;
+    const int64_t blocks = p.tiles_m * p.tiles_n * p.splits;
     static_assert(Tiles<PLANES>::list[TILE].bm == BM && Tiles<PLANES>::list[TILE].bn == BN, "the plan's tile");
     SLIM_REQUIRE(blocks * 64 * WM * WN < (int64_t)1 << 32 && blocks < 0x7fffffff, "gemm8: the result is too large for one launch");
-    auto kernel = gemm8_kernel<PLANES, FM, FN, WM, WN, STAGES, OCC, REST>;
+    auto kernel = gemm8_kernel<PLANES, FM, FN, WM, WN, STAGES, OCC>;
     SLIM_HIP(slim_allow_dynamic_lds((const void*)kernel, bytes));
     kernel<<<(unsigned)blocks, 64 * WM * WN, bytes, st>>>(g);
+    SLIM_LAUNCH_CHECK();
+    return SLIM_OK;
+}
+
+template <int PLANES, int FM, int REST>
+int launch_stream8(const Gemm8Args& g, const Plan& p, hipStream_t st) {
+    constexpr int bytes = (32 * FM + 256) * (2 * 128 + 4);
+    static_assert(Tiles<PLANES>::list[0].bm == 32 * FM && Tiles<PLANES>::list[0].bn == 256, "the plan's tile");
+    SLIM_REQUIRE(p.tiles_m * (p.tiles_n + p.rest_n) < 0x7fffffff - 256, "gemm8: the result is too large for one launch");
+    auto kernel = gemm8_stream_kernel<PLANES, FM, 4, 2, 4, REST>;
+    SLIM_HIP(slim_allow_dynamic_lds((const void*)kernel, bytes));
+    kernel<<<256, 512, bytes, st>>>(g);
     SLIM_LAUNCH_CHECK();
     return SLIM_OK;
 }
@@ -591,10 +787,11 @@ int gemm8(Gemm8Args g, void* slab, hipStream_t st) {
     g.slab = p.splits > 1 ? (int32_t*)slab : nullptr;
     int rc;
     if constexpr (PLANES == 3) {
-        rc = p.tile == 0 ? launch_gemm8<3, 0, 6, 4, 2, 4, 2, 2>(g, p, st) : launch_gemm8<3, 1, 3, 2, 2, 4, 4, 2>(g, p, st);
+        rc = p.stays() ? launch_stream8<3, 6, 0>(g, p, st) : p.tile == 0 ? launch_gemm8<3, 0, 6, 4, 2, 4, 2, 2>(g, p, st) : launch_gemm8<3, 1, 3, 2, 2, 4, 4, 2>(g, p, st);
     } else {
-        if (p.tile == 0 && p.rest == 3) rc = launch_gemm8<PLANES, 0, 8, 4, 2, 4, 2, 2, 3>(g, p, st);
-        else if (p.tile == 0 && p.rest == 2) rc = launch_gemm8<PLANES, 0, 8, 4, 2, 4, 2, 2, 2>(g, p, st);
+        if (p.stays() && p.rest == 3) rc = launch_stream8<PLANES, 8, 3>(g, p, st);
+        else if (p.stays() && p.rest == 2) rc = launch_stream8<PLANES, 8, 2>(g, p, st);
+        else if (p.stays()) rc = launch_stream8<PLANES, 8, 0>(g, p, st);
         else if (p.tile == 0) rc = launch_gemm8<PLANES, 0, 8, 4, 2, 4, 2, 2>(g, p, st);
         else if (p.tile == 1) rc = launch_gemm8<PLANES, 1, 4, 4, 2, 4, 3, 2>(g, p, st);
         else if (p.tile == 2) rc = launch_gemm8<PLANES, 2, 4, 2, 2, 4, 4, 2>(g, p, st);

@@ -396,3 +396,40 @@ def test_offsets_beyond_32_bits(ops):
         assert sampled_rows_equal(ops, y[:, :600], x, codes[:600], scale[:600], None, [0, M - 1])
     t = ops.transpose8(codes[:, :128 * 7].contiguous(), 128 * 7 - 5)
     assert torch.equal(t[:, :N], codes[:, :128 * 7 - 5].t()) and not bool(t[:, N:].any())
+
+
+# more 256 x 256 (192 x 256) tiles than CUs: workgroups that take several, with two steps and with one, all tiles whole or not, with and
+# without a last round of narrower ones
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(4096, 8192, 256), (4090, 8190, 130), (4096, 8192, 100), (1200, 25500, 260), (2600, 9000, 1100), (8200, 4352, 500)])
+def test_workgroups_with_several_tiles(ops, M, N, K, dtype):
+    test_large_products_against_64_bits(ops, M, N, K, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(2048, 256, 8192), (2050, 130, 8190), (2048, 100, 8192), (2100, 700, 9001)])
+def test_gradient_workgroups_with_several_tiles(ops, M, N, K, dtype):
+    test_large_gradients_against_64_bits(ops, M, N, K, dtype)
+
+
+def test_several_tiles_captured_and_on_two_streams(ops):
+    a, b = random_codes(2600, 1100, 5).to(DEV), random_codes(9000, 1100, 6).to(DEV)
+    sa, sb = torch.rand(2600, device=DEV), torch.rand(9000, device=DEV)
+    want = ops.gemm8_nt(a, sa, b, sb)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.gemm8_nt(a, sa, b, sb)
+    for i in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(ops.gemm8_nt(a, sa, b, sb))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
