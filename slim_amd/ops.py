@@ -1279,10 +1279,14 @@ def _plain(groups, index):
     """Whether every (tensors, type, sizes or None) holds contiguous tensors of its type and sizes on GPU `index` (a quick check: an
     optimizer step may have thousands of tensors; _alike says what is wrong)."""
     cls = torch.Tensor
-    tensors = [t for g in groups for t in g[0]]
+    numel, tensors, types = cls.numel, [], []
     try:
-        return (set(map(cls.get_device, tensors)) == {index} and all(map(cls.is_contiguous, tensors)) and
-                all(set(map(_dtype_of, ts)) == {dtype} and (sizes is None or list(map(cls.numel, ts)) == sizes) for ts, dtype, sizes in groups))
+        for ts, dtype, sizes in groups:
+            if sizes is not None and [*map(numel, ts)] != sizes:
+                return False
+            tensors += ts
+            types += [dtype] * len(ts)
+        return {*map(cls.get_device, tensors)} == {index} and all(map(cls.is_contiguous, tensors)) and [*map(_dtype_of, tensors)] == types
     except (TypeError, RuntimeError, AttributeError):
         return False
 
@@ -1334,13 +1338,12 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, beta1=0.9, bet
     params, grads, ms, vs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
     ss, ws = None if scales is None else list(scales), None if masters is None else list(masters)
     count = len(params)
-    if any(x is not None and len(x) != count for x in (grads, ms, vs, ss, ws)):
+    if not count == len(grads) == len(ms) == len(vs) or ss is not None and len(ss) != count or ws is not None and len(ws) != count:
         raise ValueError("adamw_step: all lists must be equally long")
     if not count:
         return
     gpu = _gpu_of(params[0], "params")
     dtype = params[0].dtype
-    _alike(params[:1], dtype, gpu, None, "adamw_step: params")
     dt = _DTYPES.get(dtype)
     if dt is None:
         raise TypeError(f"params must be float32, bfloat16 or float16, got {dtype}")
@@ -1350,7 +1353,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, beta1=0.9, bet
         sizes = list(map(torch.Tensor.numel, params))
     except TypeError:
         sizes = None                                     # (not tensors: the checks below say so)
-    groups = [(params, dtype, sizes), (grads, dtype, sizes), (ms, torch.float32 if ss is None else torch.float8_e4m3fn, sizes),
+    groups = [(params, dtype, None), (grads, dtype, sizes), (ms, torch.float32 if ss is None else torch.float8_e4m3fn, sizes),
               (vs, torch.float32 if ss is None else torch.float8_e5m2, sizes)]
     names = ["params", "grads", "exp_avgs", "exp_avg_sqs"]
     if ss is not None:
@@ -1372,8 +1375,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, beta1=0.9, bet
         sizes = [sizes[i] for i in keep]
         if not keep:
             return
-    lists = [x for x in (grads, params, ms, vs, ss, ws) if x is not None]
-    addresses = [a for x in lists for a in map(torch.Tensor.data_ptr, x)]
+    addresses = [*map(torch.Tensor.data_ptr, itertools.chain(grads, params, ms, vs, ss or (), ws or ()))]
     if len(set(addresses[len(grads):])) < len(addresses) - len(grads):
         raise ValueError("adamw_step: a tensor that is updated is in the lists twice")
     words, at = _words(itertools.chain(addresses, sizes))                # one array after another
@@ -1381,4 +1383,4 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, beta1=0.9, bet
     arrays = [None if x is None else next(starts) for x in (grads, params, ms, vs, ss, ws)] + [next(starts)]
     _call_at(gpu, "slim_adamw_step", arrays[1], arrays[0], *arrays[2:], len(params), dt, int(first_index), int(step), float(lr), float(beta1), float(beta2), float(eps),
              float(weight_decay), _p(norm), 0.0 if max_norm is None else float(max_norm), int(seed) & 0xffffffff)
-    torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])
+    torch.autograd.graph.increment_version(params)
