@@ -812,38 +812,40 @@ int gemm8(Gemm8Args g, void* slab, hipStream_t st) {
 // barrier is that in front of the sums' addition.  (Loaded straight into the matrix instructions' layout, 16 rows by 64 bytes a
 // request, the weight takes half as long again.)
 struct RingArgs {
-    const int8_t* A;                                     // codes of the tokens
-    int64_t lda;
+    const int8_t* A;                                     // codes of the tokens (planes interleaved when PLANES > 1)
+    int64_t lda, rows;
     const float* sa;
     const int8_t* B;
     int64_t ldb;
-    const float* sb;
+    const float* sb;                                     // or null
     const void* bias;
     void* out;
     int64_t ldo;
-    int dtype, M, N, units;
+    int dtype;
+    int64_t M, N;
+    int units;
 };
-template <int FM, int FN, int NW, int STAGES>
+template <int PLANES, int FM, int FN, int NW, int STAGES>
 __global__ __launch_bounds__(64 * NW) void ring8_kernel(const RingArgs g) {
     constexpr int REQ = 2 * FM + 2 * FN, UNIT = REQ * 1024;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
-    const int64_t n0 = (int64_t)blockIdx.x * 16 * FN;
+    const int64_t n0 = (int64_t)blockIdx.x * 16 * FN, r0 = (int64_t)blockIdx.y * 16 * FM, m0 = r0 / PLANES;
     char* const ring = lds + wave * STAGES * UNIT;
     uint32_t off[REQ];                                   // a request: eight rows, lane / 8, of which it takes piece (lane % 8) ^ row
     {
         const int pr = lane >> 3, pc = (lane & 7) ^ pr;
 #pragma unroll
         for (int s = 0; s < REQ; ++s)
-            off[s] = (s < 2 * FM ? (uint32_t)(min(s * 8 + pr, g.M - 1) * g.lda) : (uint32_t)(min((int64_t)(s - 2 * FM) * 8 + pr, g.N - 1 - n0) * g.ldb)) + pc * 16;
+            off[s] = (s < 2 * FM ? (uint32_t)(min((int64_t)s * 8 + pr, g.rows - 1 - r0) * g.lda) : (uint32_t)(min((int64_t)(s - 2 * FM) * 8 + pr, g.N - 1 - n0) * g.ldb)) + pc * 16;
     }
-    const int8_t* const b0 = g.B + n0 * g.ldb;
+    const int8_t *const a0 = g.A + r0 * g.lda, *const b0 = g.B + n0 * g.ldb;
     const int mine = wave < g.units ? (g.units - wave + NW - 1) / NW : 0;
     auto request = [&](int i, int stage) {
         const int64_t k = (int64_t)(wave + i * NW) * 128;
 #pragma unroll
         for (int s = 0; s < REQ; ++s)
-            __builtin_amdgcn_global_load_lds((glb_ptr_t)((s < 2 * FM ? g.A : b0) + k + off[s]), (lds_ptr_t)(ring + stage * UNIT + s * 1024), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((glb_ptr_t)((s < 2 * FM ? a0 : b0) + k + off[s]), (lds_ptr_t)(ring + stage * UNIT + s * 1024), 16, 0, 0);
     };
 #pragma unroll
     for (int i = 0; i < STAGES; ++i)
@@ -886,25 +888,30 @@ __global__ __launch_bounds__(64 * NW) void ring8_kernel(const RingArgs g) {
         for (int j = 0; j < FN; ++j) sums[(i * FN + j) * 64 + lane] = acc[i][j];
     __syncthreads();
     // a result per thread and turn: channel n of token m (the instruction's rows are channels, its columns tokens)
-    for (int t = threadIdx.x; t < 256 * FM * FN; t += 64 * NW) {
+    for (int t = threadIdx.x; t < 256 * FM / PLANES * FN; t += 64 * NW) {
         const int n = t % (16 * FN), m = t / (16 * FN);
-        if (m >= g.M || n0 + n >= g.N) continue;
-        const int at = ((m >> 4) * FN + (n >> 4)) * 64 + ((n & 15) >> 2) * 16 + (m & 15);
-        int sum = 0;
+        if (m0 + m >= g.M || n0 + n >= g.N) continue;
+        int sum[PLANES];
 #pragma unroll
-        for (int w = 0; w < NW; ++w) sum += ((const int*)(lds + w * STAGES * UNIT))[at * 4 + (n & 3)];
-        float v = ((float)sum * g.sa[m]) * g.sb[n0 + n];
+        for (int p = 0; p < PLANES; ++p) {
+            const int at = (((m >> 4) * PLANES + p) * FN + (n >> 4)) * 64 + ((n & 15) >> 2) * 16 + (m & 15);
+            sum[p] = 0;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) sum[p] += ((const int*)(lds + w * STAGES * UNIT))[at * 4 + (n & 3)];
+        }
+        float v = (join_planes<PLANES>(sum, 1) * g.sa[m0 + m]) * (g.sb ? g.sb[n0 + n] : 1.f);
         if (g.bias) v += load_as_f32(g.bias, n0 + n, g.dtype);
-        store_as(g.out, m * g.ldo + n0 + n, g.dtype, v);
+        store_as(g.out, (m0 + m) * g.ldo + n0 + n, g.dtype, v);
     }
 }
 
-template <int FM, int FN, int NW, int STAGES>
+template <int PLANES, int FM, int FN, int NW, int STAGES>
 int launch_ring8_as(const RingArgs& g, hipStream_t st) {
     constexpr int bytes = NW * STAGES * (FM + FN) * 2048;
-    auto kernel = ring8_kernel<FM, FN, NW, STAGES>;
+    static_assert(FM % PLANES == 0, "a workgroup holds whole groups of planes");
+    auto kernel = ring8_kernel<PLANES, FM, FN, NW, STAGES>;
     SLIM_HIP(slim_allow_dynamic_lds((const void*)kernel, bytes));
-    kernel<<<(unsigned)ceil_div64(g.N, 16 * FN), 64 * NW, bytes, st>>>(g);
+    kernel<<<dim3((unsigned)ceil_div64(g.N, 16 * FN), (unsigned)ceil_div64(g.rows, 16 * FM)), 64 * NW, bytes, st>>>(g);
     SLIM_LAUNCH_CHECK();
     return SLIM_OK;
 }
@@ -912,13 +919,27 @@ int launch_ring8_as(const RingArgs& g, hipStream_t st) {
 // eight waves 7.0, 13.8 and 21.5 for 16 tokens, 32 channels and four waves 8.0, 11.5 and 18.0; 8.2, 15.8 and 24.3 against 8.9, 13.5 and
 // 19.2 for 32.  From 33 tokens on and with many channels the tiles above share the tokens' codes better (64 x 11008 x 4096: 16.8
 // against 20.3, but 64 x 5120 x 13824: 27.2 against 24.4).
-bool takes_ring(int64_t M, int64_t N) { return M <= 32 || (M <= 64 && N <= 8192); }
+// Small results of any number of rows go the same way, while a workgroup of 16 rows of planes (32 of plain codes) by sixteen channels each
+// finds a CU: the waves share a short reduction, where a tile walks it step by step.
+template <int PLANES>
+bool takes_ring(int64_t M, int64_t N) {
+    if (PLANES == 1 && (M <= 32 || (M <= 64 && N <= 8192))) return true;
+    return ceil_div64(M, PLANES == 1 ? 32 : 16) * ceil_div64(N, 16) <= 256;
+}
+template <int PLANES>
 int launch_ring8(const RingArgs& g, hipStream_t st) {
-    SLIM_PROF("ring8", st, (double)(g.N + g.M) * g.units * 128 + (double)g.M * g.N * element_size(g.dtype), 2.0 * g.M * g.N * g.units * 128);
-    const bool narrow = g.N <= 4096;
-    if (g.M <= 16) return narrow ? launch_ring8_as<1, 1, 8, 3>(g, st) : launch_ring8_as<1, 2, 4, 3>(g, st);
-    if (g.M <= 32) return narrow ? launch_ring8_as<2, 1, 8, 2>(g, st) : launch_ring8_as<2, 2, 4, 2>(g, st);
-    return narrow ? launch_ring8_as<4, 1, 8, 2>(g, st) : launch_ring8_as<4, 2, 4, 2>(g, st);
+    SLIM_PROF("ring8", st, (double)(g.N + g.rows) * g.units * 128 + (double)g.M * g.N * element_size(g.dtype), 2.0 * g.rows * g.N * g.units * 128);
+    if constexpr (PLANES == 3) {
+        return launch_ring8_as<3, 3, 1, 8, 2>(g, st);
+    } else if constexpr (PLANES == 2) {
+        return launch_ring8_as<2, 2, 1, 8, 3>(g, st);
+    } else {
+        const bool narrow = g.N <= 4096;
+        if (g.M <= 16) return narrow ? launch_ring8_as<1, 1, 1, 8, 3>(g, st) : launch_ring8_as<1, 1, 2, 4, 3>(g, st);
+        if (g.M <= 32) return narrow ? launch_ring8_as<1, 2, 1, 8, 2>(g, st) : launch_ring8_as<1, 2, 2, 4, 2>(g, st);
+        if (g.M <= 64) return narrow ? launch_ring8_as<1, 4, 1, 8, 2>(g, st) : launch_ring8_as<1, 4, 2, 4, 2>(g, st);
+        return launch_ring8_as<1, 2, 1, 8, 2>(g, st);
+    }
 }
 
 // ---- one or two tokens ----------------------------------------------------------------------------------------------
@@ -1121,7 +1142,7 @@ extern "C" int slim_transpose8(const int8_t* codes, int64_t N, int64_t K, int64_
 }
 
 extern "C" int64_t slim_gemm8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    return M > 0 && N > 0 && K > 0 && !takes_ring(M, N) ? plan_gemm8<1>(M, N, pad128(K) / 128).slab_bytes() : 0;
+    return M > 0 && N > 0 && K > 0 && !takes_ring<1>(M, N) ? plan_gemm8<1>(M, N, pad128(K) / 128).slab_bytes() : 0;
 }
 
 extern "C" int slim_gemm8_nt(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, const float* sb, int64_t M, int64_t N,
@@ -1134,7 +1155,7 @@ extern "C" int slim_gemm8_nt(const int8_t* a, int64_t lda, const float* sa, cons
     SLIM_REQUIRE(workspace_bytes >= slim_gemm8_workspace_bytes(M, N, K) && (workspace || workspace_bytes == 0) && (uintptr_t)workspace % 16 == 0,
                  "slim_gemm8_nt: workspace too small or misaligned");
     SLIM_REQUIRE(lda < 1 << 23 && ldb < 1 << 23, "slim_gemm8_nt: rows of codes lie too far apart");
-    if (takes_ring(M, N)) return launch_ring8(RingArgs{a, lda, sa, b, ldb, sb, bias, out, ldo, dtype, (int)M, (int)N, (int)(pad128(K) / 128)}, (hipStream_t)stream);
+    if (takes_ring<1>(M, N)) return launch_ring8<1>(RingArgs{a, lda, M, sa, b, ldb, sb, bias, out, ldo, dtype, M, N, (int)(pad128(K) / 128)}, (hipStream_t)stream);
     Gemm8Args g{a, b, lda, ldb, M, M, N, (int)(pad128(K) / 128), sa, sb, bias, out, ldo, dtype, 0, 0, 1, 0, nullptr, 0};
     return gemm8<1>(g, workspace, (hipStream_t)stream);
 }
@@ -1168,7 +1189,9 @@ extern "C" int slim_linear8_forward(const void* x, int dtype, int64_t ldx, int64
 extern "C" int64_t slim_linear8_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
     if (M <= 0 || N <= 0 || K <= 0 || !known(dtype)) return 0;
     const int64_t rows = (M + 15) / 16 * 16 * planes_of(dtype);
-    return align256(rows * pad128(N)) + align256(M * 4) + (planes_of(dtype) == 3 ? plan_gemm8<3>(rows, K, pad128(N) / 128) : plan_gemm8<2>(rows, K, pad128(N) / 128)).slab_bytes();
+    const bool ring = planes_of(dtype) == 3 ? takes_ring<3>(M, K) : takes_ring<2>(M, K);
+    return align256(rows * pad128(N)) + align256(M * 4) +
+           (ring ? 0 : (planes_of(dtype) == 3 ? plan_gemm8<3>(rows, K, pad128(N) / 128) : plan_gemm8<2>(rows, K, pad128(N) / 128)).slab_bytes());
 }
 
 extern "C" int slim_linear8_backward(const void* dy, int dtype, int64_t lddy, int64_t M, int64_t N, const int8_t* codes_t, const float* scale, int64_t K,
@@ -1187,6 +1210,10 @@ extern "C" int slim_linear8_backward(const void* dy, int dtype, int64_t lddy, in
     const int rc = planes == 3 ? quantize_rows_any<3>(dy, dtype, M, N, lddy, scale, q, ld, sq, st)
                                : quantize_rows_any<2>(dy, dtype, M, N, lddy, scale, q, ld, sq, st);
     if (rc) return rc;
+    if (planes == 3 ? takes_ring<3>(M, K) : takes_ring<2>(M, K)) {
+        const RingArgs g{q, ld, rows, sq, codes_t, ld, nullptr, nullptr, dx, lddx, dtype, M, K, (int)(ld / 128)};
+        return planes == 3 ? launch_ring8<3>(g, st) : launch_ring8<2>(g, st);
+    }
     void* slab = (char*)sq + align256(M * 4);
     Gemm8Args g{q, codes_t, ld, ld, rows, M, K, (int)(ld / 128), sq, nullptr, nullptr, dx, lddx, dtype, 0, 0, 1, 0, nullptr, 0};
     return planes == 3 ? gemm8<3>(g, slab, st) : gemm8<2>(g, slab, st);
