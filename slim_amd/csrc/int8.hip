@@ -915,30 +915,36 @@ int launch_ring8_as(const RingArgs& g, hipStream_t st) {
     SLIM_LAUNCH_CHECK();
     return SLIM_OK;
 }
-// Measured over both (us with the tokens' quantisation, weights 4096 x 4096, 11008 x 4096 and 5120 x 13824): sixteen channels and
-// eight waves 7.0, 13.8 and 21.5 for 16 tokens, 32 channels and four waves 8.0, 11.5 and 18.0; 8.2, 15.8 and 24.3 against 8.9, 13.5 and
-// 19.2 for 32.  From 33 tokens on and with many channels the tiles above share the tokens' codes better (64 x 11008 x 4096: 16.8
-// against 20.3, but 64 x 5120 x 13824: 27.2 against 24.4).
-// Small results of any number of rows go the same way, while a workgroup of 16 rows of planes (32 of plain codes) by sixteen channels each
-// finds a CU: the waves share a short reduction, where a tile walks it step by step.
+// Up to 32 tokens, measured over both (us with the tokens' quantisation, weights 4096 x 4096, 11008 x 4096 and 5120 x 13824): sixteen
+// channels and eight waves 7.0, 13.8 and 21.5 for 16 tokens, 32 channels and four waves 8.0, 11.5 and 18.0; 8.2, 15.8 and 24.3 against
+// 8.9, 13.5 and 19.2 for 32.  From 33 to 64 all rows in one workgroup and eight waves where two to a CU would fill the chip (40 x 4096
+// x 11008: 12.8 against 15.4; but 64 x 1024 x 1024 3.7 against 3.2).
+// Small results of more rows, and the planes of gradients, go the same way while every workgroup finds a place at once: four waves
+// share a reduction that a tile walks step by step (rows x channels x reduction, us, tile / here: 128 x 512 x 2048 7.5 / 3.6, 512 x
+// 512 x 8192 14.6 / 11.8; gradients with their quantisation: 77 x 776 x 1000 fp32 9.6 / 6.7, 64 x 1024 x 2048 bf16 11.7 / 7.7).  First in
+// workgroups of 32 rows of codes by sixteen channels (planes: sixteen rows of the result), two a CU, then in four times that, one a CU
+// (128 x 4096 x 2048 7.6 / 6.4, gradient 256 x 1024 x 2048 bf16 12.6 / 11.2); with more of them the tiles win (512 workgroups of the
+// second: 1024 x 1024 x 2048 8.1 / 11.5).
 template <int PLANES>
-bool takes_ring(int64_t M, int64_t N) {
-    if (PLANES == 1 && (M <= 32 || (M <= 64 && N <= 8192))) return true;
-    return ceil_div64(M, PLANES == 1 ? 32 : 16) * ceil_div64(N, 16) <= 256;
+int takes_ring(int64_t M, int64_t N) {                   // 0: no; 1, 2: the smaller or the larger workgroups
+    constexpr int rows = PLANES == 1 ? 32 : 16;
+    if (PLANES == 1 && M <= 32) return 1;
+    return ceil_div64(M, rows) * ceil_div64(N, 16) <= 512 ? 1 : ceil_div64(M, 2 * rows) * ceil_div64(N, 32) <= 256 ? 2 : 0;
 }
 template <int PLANES>
 int launch_ring8(const RingArgs& g, hipStream_t st) {
     SLIM_PROF("ring8", st, (double)(g.N + g.rows) * g.units * 128 + (double)g.M * g.N * element_size(g.dtype), 2.0 * g.rows * g.N * g.units * 128);
+    const bool large = takes_ring<PLANES>(g.M, g.N) == 2;
     if constexpr (PLANES == 3) {
-        return launch_ring8_as<3, 3, 1, 8, 2>(g, st);
+        return large ? launch_ring8_as<3, 6, 2, 4, 2>(g, st) : launch_ring8_as<3, 3, 1, 4, 2>(g, st);
     } else if constexpr (PLANES == 2) {
-        return launch_ring8_as<2, 2, 1, 8, 3>(g, st);
+        return large ? launch_ring8_as<2, 4, 2, 4, 3>(g, st) : launch_ring8_as<2, 2, 1, 4, 3>(g, st);
     } else {
         const bool narrow = g.N <= 4096;
         if (g.M <= 16) return narrow ? launch_ring8_as<1, 1, 1, 8, 3>(g, st) : launch_ring8_as<1, 1, 2, 4, 3>(g, st);
         if (g.M <= 32) return narrow ? launch_ring8_as<1, 2, 1, 8, 2>(g, st) : launch_ring8_as<1, 2, 2, 4, 2>(g, st);
-        if (g.M <= 64) return narrow ? launch_ring8_as<1, 4, 1, 8, 2>(g, st) : launch_ring8_as<1, 4, 2, 4, 2>(g, st);
-        return launch_ring8_as<1, 2, 1, 8, 2>(g, st);
+        if (g.M <= 64 && narrow && g.N > 2048) return launch_ring8_as<1, 4, 1, 8, 2>(g, st);
+        return large ? launch_ring8_as<1, 4, 2, 4, 3>(g, st) : launch_ring8_as<1, 2, 1, 4, 3>(g, st);
     }
 }
 

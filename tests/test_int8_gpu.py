@@ -433,3 +433,17 @@ def test_several_tiles_captured_and_on_two_streams(ops):
                 outs.append(ops.gemm8_nt(a, sa, b, sb))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+# small results on wave-private rings: the borders of the smaller and the larger workgroups, reductions of one unit, fewer and more
+# than the waves take at once
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(33, 17, 100), (512, 512, 300), (513, 511, 640), (255, 2047, 1700), (257, 2048, 130), (100, 1000, 5000), (1025, 100, 900), (4000, 33, 500)])
+def test_small_results_against_64_bits(ops, M, N, K, dtype):
+    test_large_products_against_64_bits(ops, M, N, K, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 100, 17), (128, 300, 1024), (129, 640, 1023), (255, 1700, 1024), (257, 130, 1024), (16, 5000, 4097), (33, 4000, 700), (1025, 900, 100), (4000, 500, 33)])
+def test_small_gradients_against_64_bits(ops, M, N, K, dtype):
+    test_large_gradients_against_64_bits(ops, M, N, K, dtype)
