@@ -1108,9 +1108,10 @@ def _rows8(t, name):
     code = _DTYPES.get(t.dtype)
     if code is None:
         raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-    if t.dim() != 2 or t.size(1) == 0:
-        raise ValueError(f"{name} must be a matrix with at least one column, got {tuple(t.shape)}")
-    rows, cols = t.shape
+    shape = t.shape
+    if len(shape) != 2 or shape[1] == 0:
+        raise ValueError(f"{name} must be a matrix with at least one column, got {tuple(shape)}")
+    rows, cols = shape
     if t.is_contiguous():
         return t, rows, cols, cols, code, index
     if cols > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < cols:
@@ -1135,9 +1136,10 @@ def _operand(t, dtype, index, name):
 def _codes8(t, index, name):
     """A contiguous int8 matrix of codes and its shape."""
     t = _operand(t, torch.int8, index, name)
-    if t.dim() != 2 or t.numel() == 0 or t.size(1) % 128:
-        raise ValueError(f"{name} must be [rows, a multiple of 128], got {tuple(t.shape)}")
-    return t, t.size(0), t.size(1)
+    shape = t.shape
+    if len(shape) != 2 or shape[0] == 0 or shape[1] == 0 or shape[1] % 128:
+        raise ValueError(f"{name} must be [rows, a multiple of 128], got {tuple(shape)}")
+    return t, shape[0], shape[1]
 
 
 def _vector(t, n, dtype, index, name):
@@ -1145,6 +1147,11 @@ def _vector(t, n, dtype, index, name):
     if t.numel() != n:
         raise ValueError(f"{name} must hold {n} values, got {tuple(t.shape)}")
     return t
+
+
+def _matrix(rows, cols, dtype, device):
+    """torch.empty((rows, cols)), which takes a quarter longer (1.7 us)."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
 
 
 def _pad128(k):
@@ -1165,7 +1172,7 @@ def quantize_rows8(x):
     everywhere gets scale 0; one that holds an infinity or a NaN gets scale NaN.  Tokens of an activation, or output channels
     of a weight [N, K] (the operand of linear8_forward)."""
     x, R, K, ld, dt, gpu = _rows8(x, "x")
-    codes = torch.empty((R, _pad128(K)), dtype=torch.int8, device=x.device)
+    codes = _matrix(R, _pad128(K), torch.int8, x.device)
     scale = torch.empty(R, dtype=torch.float32, device=x.device)
     if R:
         _call_at(gpu, "slim_quantize_rows8", x.data_ptr(), dt, R, K, ld, codes.data_ptr(), _pad128(K), scale.data_ptr())
@@ -1205,7 +1212,7 @@ def gemm8_nt(a, sa, b, sb, bias=None, out_dtype=BF16, K=None):
     sa, sb = _vector(sa, M, torch.float32, gpu, "sa"), _vector(sb, N, torch.float32, gpu, "sb")
     if bias is not None:
         bias = _vector(bias, N, out_dtype, gpu, "bias")
-    out = torch.empty((M, N), dtype=out_dtype, device=a.device)
+    out = _matrix(M, N, out_dtype, a.device)
     need = _lib.query("slim_gemm8_workspace_bytes", M, N, K)
     ws = _workspace(need, a.device)
     _call_at(gpu, "slim_gemm8_nt", a.data_ptr(), Kp, sa.data_ptr(), b.data_ptr(), Kp, sb.data_ptr(), M, N, K, _p(bias), _DTYPES[out_dtype], out.data_ptr(), N,
@@ -1223,7 +1230,7 @@ def linear8_forward(x, codes, scale, bias=None):
     scale = _vector(scale, N, torch.float32, gpu, "scale")
     if bias is not None:
         bias = _vector(bias, N, x.dtype, gpu, "bias")
-    y = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    y = _matrix(M, N, x.dtype, x.device)
     if M:
         need = _lib.query("slim_linear8_workspace_bytes", M, N, K)
         ws = _workspace(need, x.device)
@@ -1240,7 +1247,7 @@ def linear8_backward(dy, codes_t, scale):
     if Np != _pad128(N):
         raise ValueError(f"codes_t of a weight with {N} output channels has {_pad128(N)} columns, got {Np}")
     scale = _vector(scale, N, torch.float32, gpu, "scale")
-    dx = torch.empty((M, K), dtype=dy.dtype, device=dy.device)
+    dx = _matrix(M, K, dy.dtype, dy.device)
     if M:
         need = _lib.query("slim_linear8_backward_workspace_bytes", M, N, K, dt)
         ws = _workspace(need, dy.device)
