@@ -67,8 +67,7 @@ __device__ __forceinline__ RowScale row_scale(uint32_t max_bits) {
 }
 
 template <int PLANES>
-__device__ __forceinline__ void store_codes(const float x[8], float r, int8_t* codes, int64_t ldc, int64_t row, int64_t col) {
-    uint32_t out[PLANES][2];
+__device__ __forceinline__ void encode(const float x[8], float r, uint32_t (&out)[PLANES][2]) {
 #pragma unroll
     for (int p = 0; p < PLANES; ++p) out[p][0] = out[p][1] = 0;
 #pragma unroll
@@ -83,6 +82,11 @@ __device__ __forceinline__ void store_codes(const float x[8], float r, int8_t* c
             q = (q - low) >> 8;
         }
     }
+}
+template <int PLANES>
+__device__ __forceinline__ void store_codes(const float x[8], float r, int8_t* codes, int64_t ldc, int64_t row, int64_t col) {
+    uint32_t out[PLANES][2];
+    encode<PLANES>(x, r, out);
 #pragma unroll
     for (int p = 0; p < PLANES; ++p) {
         const int64_t at = PLANES == 1 ? row : ((row >> 4) * PLANES + p) * 16 + (row & 15);
@@ -825,6 +829,26 @@ struct RingArgs {
     int64_t M, N;
     int units;
 };
+// The waves' sums, `stride` bytes from one wave's to the next, added: a result per thread and turn, channel n of token m (the
+// instruction's rows are channels, its columns tokens).  sa: the scales of the workgroup's tokens.
+template <int PLANES, int FM, int FN, int NW>
+__device__ __forceinline__ void wave_results(const RingArgs& g, const char* sums, int stride, const float* sa, int64_t m0, int64_t n0) {
+    for (int t = threadIdx.x; t < 256 * FM / PLANES * FN; t += 64 * NW) {
+        const int n = t % (16 * FN), m = t / (16 * FN);
+        if (m0 + m >= g.M || n0 + n >= g.N) continue;
+        int sum[PLANES];
+#pragma unroll
+        for (int p = 0; p < PLANES; ++p) {
+            const int at = (((m >> 4) * PLANES + p) * FN + (n >> 4)) * 64 + ((n & 15) >> 2) * 16 + (m & 15);
+            sum[p] = 0;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) sum[p] += ((const int*)(sums + w * stride))[at * 4 + (n & 3)];
+        }
+        float v = (join_planes<PLANES>(sum, 1) * sa[m]) * (g.sb ? g.sb[n0 + n] : 1.f);
+        if (g.bias) v += load_as_f32(g.bias, n0 + n, g.dtype);
+        store_as(g.out, (m0 + m) * g.ldo + n0 + n, g.dtype, v);
+    }
+}
 template <int PLANES, int FM, int FN, int NW, int STAGES>
 __global__ __launch_bounds__(64 * NW) void ring8_kernel(const RingArgs g) {
     constexpr int REQ = 2 * FM + 2 * FN, UNIT = REQ * 1024;
@@ -887,22 +911,7 @@ __global__ __launch_bounds__(64 * NW) void ring8_kernel(const RingArgs g) {
 #pragma unroll
         for (int j = 0; j < FN; ++j) sums[(i * FN + j) * 64 + lane] = acc[i][j];
     __syncthreads();
-    // a result per thread and turn: channel n of token m (the instruction's rows are channels, its columns tokens)
-    for (int t = threadIdx.x; t < 256 * FM / PLANES * FN; t += 64 * NW) {
-        const int n = t % (16 * FN), m = t / (16 * FN);
-        if (m0 + m >= g.M || n0 + n >= g.N) continue;
-        int sum[PLANES];
-#pragma unroll
-        for (int p = 0; p < PLANES; ++p) {
-            const int at = (((m >> 4) * PLANES + p) * FN + (n >> 4)) * 64 + ((n & 15) >> 2) * 16 + (m & 15);
-            sum[p] = 0;
-#pragma unroll
-            for (int w = 0; w < NW; ++w) sum[p] += ((const int*)(lds + w * STAGES * UNIT))[at * 4 + (n & 3)];
-        }
-        float v = (join_planes<PLANES>(sum, 1) * g.sa[m0 + m]) * (g.sb ? g.sb[n0 + n] : 1.f);
-        if (g.bias) v += load_as_f32(g.bias, n0 + n, g.dtype);
-        store_as(g.out, (m0 + m) * g.ldo + n0 + n, g.dtype, v);
-    }
+    wave_results<PLANES, FM, FN, NW>(g, lds, STAGES * UNIT, g.sa + m0, m0, n0);
 }
 
 template <int PLANES, int FM, int FN, int NW, int STAGES>
@@ -921,7 +930,7 @@ int launch_ring8_as(const RingArgs& g, hipStream_t st) {
 // x 11008: 12.8 against 15.4; but 64 x 1024 x 1024 3.7 against 3.2).
 // Small results of more rows, and the planes of gradients, go the same way while every workgroup finds a place at once: four waves
 // share a reduction that a tile walks step by step (rows x channels x reduction, us, tile / here: 128 x 512 x 2048 7.5 / 3.6, 512 x
-// 512 x 8192 14.6 / 11.8; gradients with their quantisation: 77 x 776 x 1000 fp32 9.6 / 6.7, 64 x 1024 x 2048 bf16 11.7 / 7.7).  First in
+// 512 x 8192 14.6 / 11.8; gradients with their quantisation: 16 x 4096 x 4096 fp32 15.8 / 10.4, 64 x 1024 x 2048 bf16 11.7 / 7.7).  First in
 // workgroups of 32 rows of codes by sixteen channels (planes: sixteen rows of the result), two a CU, then in four times that, one a CU
 // (128 x 4096 x 2048 7.6 / 6.4, gradient 256 x 1024 x 2048 bf16 12.6 / 11.2); with more of them the tiles win (512 workgroups of the
 // second: 1024 x 1024 x 2048 8.1 / 11.5).
@@ -946,6 +955,117 @@ int launch_ring8(const RingArgs& g, hipStream_t st) {
         if (g.M <= 64 && narrow && g.N > 2048) return launch_ring8_as<1, 4, 1, 8, 2>(g, st);
         return large ? launch_ring8_as<1, 4, 2, 4, 3>(g, st) : launch_ring8_as<1, 2, 1, 4, 3>(g, st);
     }
+}
+
+// ---- small products in one launch -----------------------------------------------------------------------------------
+// Sixteen rows by sixteen channels a workgroup, which quantises its rows itself (as quantize_rows_kernel does, to the same codes), two
+// rows a wave, while the weight's rows, all units at once, travel by LDS-DMA.  N / 16 workgroups repeat that: over a short reduction it
+// takes no longer than the kernel it replaces, and saves a launch and the workspace (us on the GPU, then per call from Python, two launches /
+// one: 64 x 480 x 480 5.6 / 3.9, 12.2 / 7.8; gradient of 64 x 480 x 480 bf16 5.4 / 4.5, 12.2 / 7.8).  Four waves and four rows each: 5.1 and 5.8.
+// x: [M, K], colscale: null or a factor per column (gradients).
+constexpr int SMALL_WAVES = 8;
+template <typename T, int PLANES, int NP>
+__global__ __launch_bounds__(64 * SMALL_WAVES) void small8_kernel(const RingArgs g, const T* __restrict__ x, int64_t ldx, int K, const float* __restrict__ colscale) {
+    constexpr int NW = SMALL_WAVES, EACH = 16 / NW;      // rows of a wave
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ float sa[16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * 16;
+    char* const weight = lds + g.units * PLANES * 2048;
+    {
+        const int pr = lane >> 3, pc = (lane & 7) ^ pr;
+        const int8_t* const b0 = g.B + n0 * g.ldb;
+        for (int u = wave; u < g.units; u += NW)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+                __builtin_amdgcn_global_load_lds((glb_ptr_t)(b0 + u * 128 + (uint32_t)(min((int64_t)s * 8 + pr, g.N - 1 - n0) * g.ldb) + pc * 16), (lds_ptr_t)(weight + u * 2048 + s * 1024), 16, 0, 0);
+    }
+    float v[EACH][NP][8], f[NP][8];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const int c = (i * 64 + lane) * 8;
+        if (c < K) {
+            if (PLANES > 1) load8(colscale + c, (int64_t)K - c, f[i]);
+#pragma unroll
+            for (int r = 0; r < EACH; ++r) load8(x + min(m0 + wave * EACH + r, g.M - 1) * ldx + c, (int64_t)K - c, v[r][i]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                f[i][j] = 0.f;
+#pragma unroll
+                for (int r = 0; r < EACH; ++r) v[r][i][j] = 0.f;
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < EACH; ++r) {
+        const int row = wave * EACH + r;
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (PLANES > 1) v[r][i][j] *= f[i][j];
+                top = max(top, f32_bits(v[r][i][j]) & 0x7fffffffu);
+            }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+        const RowScale rs = row_scale<PLANES>(top);
+        if (lane == 0) sa[row] = rs.scale;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int c = (i * 64 + lane) * 8;
+            if (c >= g.units * 128) continue;
+            if (rs.none) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[r][i][j] = 0.f;
+            }
+            uint32_t out[PLANES][2];
+            encode<PLANES>(v[r][i], rs.inverse, out);
+            char* const dst = lds + (c >> 7) * PLANES * 2048 + row * 128 + ((((c >> 4) & 7) ^ (row & 7)) * 16) + (c & 8);
+#pragma unroll
+            for (int p = 0; p < PLANES; ++p) *(uint2*)(dst + p * 2048) = make_uint2(out[p][0], out[p][1]);
+        }
+    }
+    wait_vmcnt<0>();                                     // this wave's units of the weight
+    __syncthreads();
+    i32x4 acc[PLANES];
+#pragma unroll
+    for (int i = 0; i < PLANES; ++i) acc[i] = i32x4{0, 0, 0, 0};
+    const int x0 = fr * 128 + (fq ^ (fr & 7)) * 16;
+    for (int u = wave; u < g.units; u += NW)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const i32x4 b = *(const i32x4*)(weight + u * 2048 + (x0 ^ (h * 64)));
+#pragma unroll
+            for (int i = 0; i < PLANES; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, *(const i32x4*)(lds + (u * PLANES + i) * 2048 + (x0 ^ (h * 64))), acc[i], 0, 0, 0);
+        }
+    __syncthreads();                                     // (no one reads the codes any more)
+#pragma unroll
+    for (int i = 0; i < PLANES; ++i) ((i32x4*)lds)[(wave * PLANES + i) * 64 + lane] = acc[i];
+    __syncthreads();
+    wave_results<PLANES, PLANES, 1, NW>(g, lds, PLANES * 1024, sa, m0, n0);
+}
+// How many workgroups may repeat a reduction of one, two or four pieces of 512 (us on the GPU, two launches / one: 512 x 512 x 512 6.2 / 6.2,
+// 3000 x 100 x 500 9.9 / 9.0 - 10.7; 64 x 2048 x 1000 6.1 / 5.8, 256 x 1024 x 1024 7.0 / 8.5; 64 x 480 x 2048 7.2 / 5.9, 128 x 1024 x 2048 7.4 /
+// 8.6; gradients: 256 x 500 x 1000 bf16 7.3 / 7.2, 500 x 512 x 200 fp32 7.9 / 8.9, 64 x 2048 x 1000 fp32 7.1 / 8.7, 77 x 776 x 1000 6.5 / 6.6,
+// 16 x 512 x 2048 7.6 / 8.5).
+template <int PLANES>
+bool takes_small(int64_t M, int64_t N, int64_t K) {
+    if (K > (PLANES == 1 ? 2048 : 1024)) return false;
+    const int64_t pieces = K <= 512 ? 1 : K <= 1024 ? 2 : 4, most = PLANES == 1 ? 1024 / pieces : PLANES == 2 ? 512 : 512 / pieces;
+    return ceil_div64(M, 16) * ceil_div64(N, 16) <= most;
+}
+template <typename T, int PLANES>
+int launch_small8(const RingArgs& g, const T* x, int64_t ldx, int64_t K, const float* colscale, hipStream_t st) {
+    SLIM_PROF("small8", st, (double)g.M * K * sizeof(T) + (double)g.N * g.units * 128 + (double)g.M * g.N * sizeof(T), 2.0 * PLANES * g.M * g.N * K);
+    auto kernel = K <= 512 ? small8_kernel<T, PLANES, 1> : small8_kernel<T, PLANES, 2>;
+    if constexpr (PLANES == 1) kernel = K <= 1024 ? kernel : small8_kernel<T, 1, 4>;
+    const int bytes = max(g.units * (PLANES + 1) * 2048, SMALL_WAVES * PLANES * 1024);      // codes of the rows and of the channels; the waves' sums take their place
+    SLIM_HIP(slim_allow_dynamic_lds((const void*)kernel, bytes));
+    kernel<<<dim3((unsigned)ceil_div64(g.N, 16), (unsigned)ceil_div64(g.M, 16)), 64 * SMALL_WAVES, bytes, st>>>(g, x, ldx, (int)K, colscale);
+    SLIM_LAUNCH_CHECK();
+    return SLIM_OK;
 }
 
 // ---- one or two tokens ----------------------------------------------------------------------------------------------
@@ -1167,7 +1287,7 @@ extern "C" int slim_gemm8_nt(const int8_t* a, int64_t lda, const float* sa, cons
 }
 
 extern "C" int64_t slim_linear8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    if (M <= 0 || N <= 0 || K <= 0 || token_waves(M, K)) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || token_waves(M, K) || takes_small<1>(M, N, K)) return 0;
     return align256(M * pad128(K)) + align256(M * 4) + slim_gemm8_workspace_bytes(M, N, K);
 }
 
@@ -1184,6 +1304,14 @@ extern "C" int slim_linear8_forward(const void* x, int dtype, int64_t ldx, int64
         if (dtype == SLIM_DTYPE_BF16) return token8<bf16_t>(g, M, waves, (hipStream_t)stream);
         return token8<_Float16>(g, M, waves, (hipStream_t)stream);
     }
+    if (takes_small<1>(M, N, K)) {
+        SLIM_REQUIRE(known(dtype), "slim_linear8_forward: unknown element type %d", dtype);
+        SLIM_REQUIRE(N <= SLIM_INT8_MAX_DIM && (uintptr_t)codes % 16 == 0, "slim_linear8_forward: weight too large or misaligned");
+        const RingArgs g{nullptr, 0, M, nullptr, codes, pad128(K), scale, bias, y, ldy, dtype, M, N, (int)(pad128(K) / 128)};
+        if (dtype == SLIM_DTYPE_F32) return launch_small8<float, 1>(g, (const float*)x, ldx, K, nullptr, (hipStream_t)stream);
+        if (dtype == SLIM_DTYPE_BF16) return launch_small8<bf16_t, 1>(g, (const bf16_t*)x, ldx, K, nullptr, (hipStream_t)stream);
+        return launch_small8<_Float16, 1>(g, (const _Float16*)x, ldx, K, nullptr, (hipStream_t)stream);
+    }
     int8_t* xc = (int8_t*)workspace;
     float* sx = (float*)(xc + align256(M * pad128(K)));
     const int rc = slim_quantize_rows8(x, dtype, M, K, ldx, xc, pad128(K), sx, stream);
@@ -1194,6 +1322,7 @@ extern "C" int slim_linear8_forward(const void* x, int dtype, int64_t ldx, int64
 
 extern "C" int64_t slim_linear8_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
     if (M <= 0 || N <= 0 || K <= 0 || !known(dtype)) return 0;
+    if (planes_of(dtype) == 3 ? takes_small<3>(M, K, N) : takes_small<2>(M, K, N)) return 0;
     const int64_t rows = (M + 15) / 16 * 16 * planes_of(dtype);
     const bool ring = planes_of(dtype) == 3 ? takes_ring<3>(M, K) : takes_ring<2>(M, K);
     return align256(rows * pad128(N)) + align256(M * 4) +
@@ -1202,15 +1331,22 @@ extern "C" int64_t slim_linear8_backward_workspace_bytes(int64_t M, int64_t N, i
 
 extern "C" int slim_linear8_backward(const void* dy, int dtype, int64_t lddy, int64_t M, int64_t N, const int8_t* codes_t, const float* scale, int64_t K,
                                      void* dx, int64_t lddx, void* workspace, int64_t workspace_bytes, void* stream) {
-    SLIM_REQUIRE(dy && codes_t && scale && dx && workspace && M > 0 && N > 0 && K > 0 && lddy >= N && lddx >= K, "slim_linear8_backward: bad arguments");
+    SLIM_REQUIRE(dy && codes_t && scale && dx && M > 0 && N > 0 && K > 0 && lddy >= N && lddx >= K, "slim_linear8_backward: bad arguments");
     SLIM_REQUIRE(known(dtype), "slim_linear8_backward: unknown element type %d", dtype);
     SLIM_REQUIRE(N <= SLIM_INT8_MAX_REDUCTION && M <= SLIM_INT8_MAX_DIM && K <= SLIM_INT8_MAX_DIM, "slim_linear8_backward: too large");
-    SLIM_REQUIRE(workspace_bytes >= slim_linear8_backward_workspace_bytes(M, N, K, dtype) && (uintptr_t)workspace % 16 == 0,
+    const int64_t need = slim_linear8_backward_workspace_bytes(M, N, K, dtype);
+    SLIM_REQUIRE(workspace_bytes >= need && (workspace || !need) && (uintptr_t)workspace % 16 == 0,
                  "slim_linear8_backward: workspace too small or misaligned");
     SLIM_REQUIRE((uintptr_t)codes_t % 16 == 0, "slim_linear8_backward: codes must be 16-byte aligned");
     hipStream_t st = (hipStream_t)stream;
     const int planes = planes_of(dtype);
     const int64_t rows = (M + 15) / 16 * 16 * planes, ld = pad128(N);
+    if (!need) {
+        const RingArgs g{nullptr, 0, M, nullptr, codes_t, ld, nullptr, nullptr, dx, lddx, dtype, M, K, (int)(ld / 128)};
+        if (dtype == SLIM_DTYPE_F32) return launch_small8<float, 3>(g, (const float*)dy, lddy, N, scale, st);
+        if (dtype == SLIM_DTYPE_BF16) return launch_small8<bf16_t, 2>(g, (const bf16_t*)dy, lddy, N, scale, st);
+        return launch_small8<_Float16, 2>(g, (const _Float16*)dy, lddy, N, scale, st);
+    }
     int8_t* q = (int8_t*)workspace;
     float* sq = (float*)(q + align256(rows * ld));
     const int rc = planes == 3 ? quantize_rows_any<3>(dy, dtype, M, N, lddy, scale, q, ld, sq, st)

@@ -16,10 +16,11 @@ def test_sizes():
     lib = _lib.load()
     assert [lib.slim_rows8_ld(k) for k in (1, 127, 128, 129, 4096, 0, -3)] == [128, 128, 128, 256, 4096, 0, 0]
     assert [lib.slim_adamw_blocks(n) for n in (1, 512, 513, 0)] == [1, 1, 2, 0]
-    assert lib.slim_linear8_workspace_bytes(5, 64, 100) >= 5 * 128 + 5 * 4 and lib.slim_linear8_workspace_bytes(0, 64, 100) == 0
-    assert lib.slim_linear8_workspace_bytes(1, 64, 100) == 0              # one launch, tokens quantised on the way
-    assert lib.slim_linear8_backward_workspace_bytes(5, 64, 100, 1) >= 2 * 16 * 128 + 5 * 4
-    assert lib.slim_linear8_backward_workspace_bytes(5, 64, 100, 0) >= 3 * 16 * 128 + 5 * 4
+    assert lib.slim_linear8_workspace_bytes(5, 64, 2200) >= 5 * 2304 + 5 * 4 and lib.slim_linear8_workspace_bytes(0, 64, 100) == 0
+    assert lib.slim_linear8_workspace_bytes(1, 64, 100) == lib.slim_linear8_workspace_bytes(5, 64, 100) == 0      # one launch, tokens quantised on the way
+    assert lib.slim_linear8_backward_workspace_bytes(5, 64, 100, 1) == lib.slim_linear8_backward_workspace_bytes(5, 64, 100, 0) == 0
+    assert lib.slim_linear8_backward_workspace_bytes(5, 1100, 100, 1) >= 2 * 16 * 1152 + 5 * 4
+    assert lib.slim_linear8_backward_workspace_bytes(5, 1100, 100, 0) >= 3 * 16 * 1152 + 5 * 4
     assert lib.slim_linear8_backward_workspace_bytes(5, 64, 100, 7) == 0
     assert lib.slim_grad_norm_workspace_bytes(1) > 0 and lib.slim_grad_norm_workspace_bytes(0) == 0
 
@@ -43,9 +44,9 @@ P = 1 << 20        # (an address that nothing reads: every call below is refused
     ("slim_gemm8_nt", (P, 128, P, P, 128, P, 4, 4, 128, None, 9, P, 4, None, 0, None)),
     ("slim_gemm8_nt", (P, 1 << 18, P, P, 1 << 18, P, 4, 4, 131072, None, 1, P, 4, None, 0, None)),
     ("slim_gemm8_nt", (P, 136, P, P, 128, P, 4, 4, 128, None, 1, P, 4, None, 0, None)),
-    ("slim_linear8_forward", (P, 1, 128, 4, 128, P, P, 4, None, P, 4, P, 16, None)),
+    ("slim_linear8_forward", (P, 1, 2176, 4, 2176, P, P, 4, None, P, 4, P, 16, None)),
     ("slim_linear8_forward", (P, 1, 128, 4, 128, None, P, 4, None, P, 4, P, 1 << 20, None)),
-    ("slim_linear8_backward", (P, 1, 4, 4, 4, P, P, 128, P, 128, P, 16, None)),
+    ("slim_linear8_backward", (P, 1, 1152, 4, 1152, P, P, 128, P, 128, P, 16, None)),
     ("slim_linear8_backward", (P, 1, 4, 4, 131072, P, P, 128, P, 128, P, 1 << 40, None)),
     ("slim_linear8_backward", (P, 5, 4, 4, 4, P, P, 128, P, 128, P, 1 << 20, None)),
 ])

@@ -447,3 +447,27 @@ def test_small_results_against_64_bits(ops, M, N, K, dtype):
 @pytest.mark.parametrize("M,N,K", [(1, 100, 17), (128, 300, 1024), (129, 640, 1023), (255, 1700, 1024), (257, 130, 1024), (16, 5000, 4097), (33, 4000, 700), (1025, 900, 100), (4000, 500, 33)])
 def test_small_gradients_against_64_bits(ops, M, N, K, dtype):
     test_large_gradients_against_64_bits(ops, M, N, K, dtype)
+
+
+# one launch for small products: the borders of its rule in rows, channels and reduction, ragged everywhere, views and rows that are not finite
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(3, 1, 1), (16, 16, 128), (17, 33, 129), (300, 50, 511), (512, 512, 512), (513, 512, 512), (64, 2048, 1000), (65, 2048, 1000), (255, 255, 513),
+                                   (64, 1024, 2048), (65, 1024, 2047), (7, 200, 1025), (16000, 16, 40)])
+def test_one_launch_equals_rows_then_product(ops, M, N, K, dtype):
+    x = make_rows(M, K + 3, dtype, 8).to(DEV)[:, 1:K + 1]
+    codes, scale = ops.quantize_rows8(torch.randn(N, K, device=DEV))
+    bias = torch.randn(N, device=DEV).to(dtype)
+    xc, xs = ops.quantize_rows8(x)
+    assert same(ops.linear8_forward(x, codes, scale, bias), ops.gemm8_nt(xc, xs, codes, scale, bias, dtype, K=K))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (16, 128, 16), (17, 129, 33), (300, 511, 50), (128, 512, 1024), (129, 513, 100), (256, 1024, 256), (257, 1000, 256), (512, 1024, 256), (8, 1023, 4096)])
+def test_gradients_in_one_launch(ops, M, N, K, dtype):
+    """Against 64 bits, and row by row the same as of a taller gradient, which takes other kernels."""
+    test_large_gradients_against_64_bits(ops, M, N, K, dtype)
+    w, scale = ops.quantize_rows8(torch.randn(N, K, device=DEV))
+    t = ops.transpose8(w, K)
+    dy = make_rows(9000, N, dtype, 9).to(DEV)
+    if K >= 16:
+        assert same(ops.linear8_backward(dy, t, scale)[:M], ops.linear8_backward(dy[:M], t, scale))
