@@ -555,7 +555,7 @@ int64_t slim_gemm8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int slim_gemm8_nt(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, const float* sb, int64_t M, int64_t N, int64_t K,
                   const void* bias, int dtype, void* out, int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream);
 /* y = the rows of x quantised as by slim_quantize_rows8, times the weight's codes [N, slim_rows8_ld(K)] as by slim_gemm8_nt.
- * (A workspace of 0 bytes, here one or two rows of not too many channels, may be NULL.) */
+ * (A workspace of 0 bytes, here one or two rows or a small product, may be NULL.) */
 int64_t slim_linear8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int slim_linear8_forward(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, const int8_t* codes, const float* scale, int64_t N,
                          const void* bias, void* y, int64_t ldy, void* workspace, int64_t workspace_bytes, void* stream);

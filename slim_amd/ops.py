@@ -1326,9 +1326,8 @@ def grad_norm(grads):
     norm = torch.empty((), dtype=torch.float32, device=dev)
     need = _lib.query("slim_grad_norm_workspace_bytes", len(grads))
     ws = _workspace(need, dev)
-    ptrs, ptrs_at = _words(map(torch.Tensor.data_ptr, grads))
-    counts, counts_at = _words(sizes)
-    _call_at(gpu, "slim_grad_norm", ptrs_at, counts_at, len(grads), dt, norm.data_ptr(), ws.data_ptr(), need)
+    words, at = _words([*map(torch.Tensor.data_ptr, grads)] + sizes)
+    _call_at(gpu, "slim_grad_norm", at, at + 8 * len(grads), len(grads), dt, norm.data_ptr(), ws.data_ptr(), need)
     return norm
 
 
@@ -1385,9 +1384,9 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, beta1=0.9, bet
     addresses = [*map(torch.Tensor.data_ptr, itertools.chain(grads, params, ms, vs, ss or (), ws or ()))]
     if len(set(addresses[len(grads):])) < len(addresses) - len(grads):
         raise ValueError("adamw_step: a tensor that is updated is in the lists twice")
-    words, at = _words(itertools.chain(addresses, sizes))                # one array after another
-    starts = iter(range(at, at + words.itemsize * len(words), words.itemsize * len(params)))
-    arrays = [None if x is None else next(starts) for x in (grads, params, ms, vs, ss, ws)] + [next(starts)]
-    _call_at(gpu, "slim_adamw_step", arrays[1], arrays[0], *arrays[2:], len(params), dt, int(first_index), int(step), float(lr), float(beta1), float(beta2), float(eps),
+    words, at = _words(addresses + sizes)                                # one array after another
+    size, end = 8 * len(params), at + 8 * len(addresses)
+    _call_at(gpu, "slim_adamw_step", at + size, at, at + 2 * size, at + 3 * size, None if ss is None else at + 4 * size, None if ws is None else end - size, end,
+             len(params), dt, int(first_index), int(step), float(lr), float(beta1), float(beta2), float(eps),
              float(weight_decay), _p(norm), 0.0 if max_norm is None else float(max_norm), int(seed) & 0xffffffff)
     torch.autograd.graph.increment_version(params)
