@@ -560,9 +560,10 @@ int64_t slim_linear8_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int slim_linear8_forward(const void* x, int dtype, int64_t ldx, int64_t M, int64_t K, const int8_t* codes, const float* scale, int64_t N,
                          const void* bias, void* y, int64_t ldy, void* workspace, int64_t workspace_bytes, void* stream);
 /* dx[m][k] = sum_n dy[m][n] scale[n] codes[n][k], the gradient of slim_linear8_forward with x's quantisation passed straight
- * through.  codes_t: [K, slim_rows8_ld(N)] from slim_transpose8.  dy * scale is kept per row as integers of 16 bits (24 for
- * fp32) against the row's maximum: the error of a row is at most sqrt(N / 12) * 2^-15 (2^-23) of the norm of that row.  Rows
- * that hold an infinity or a NaN give NaN.  N <= 131071. */
+ * through.  codes_t: [K, slim_rows8_ld(N)] from slim_transpose8.  v = dy * scale is an fp32 product, of which 16-bit types keep every
+ * element to 2^-23 of itself or 2^-50 of the row's largest, fp32 all bits or 2^-61; sums are fp32.  Before its rounding to the type, with
+ * D = 2^-50 (2^-61), dx[m][k] is off by at most ((N + 8) 2^-23 + 2^-24) sum_n |v[m][n] codes[n][k]| + D max_n |v[m][n]| sum_n |codes[n][k]|.
+ * Rows of v that hold an infinity or a NaN give NaN.  A row's dx does not depend on the other rows.  N <= 131071. */
 int64_t slim_linear8_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype);
 int slim_linear8_backward(const void* dy, int dtype, int64_t lddy, int64_t M, int64_t N, const int8_t* codes_t, const float* scale, int64_t K,
                           void* dx, int64_t lddx, void* workspace, int64_t workspace_bytes, void* stream);

@@ -1,106 +1,37 @@
 // Linears in 8-bit integers: rows quantised to int8 codes with one fp32 scale each (tokens of an activation, output channels
-// of a weight), the product of two such matrices on the int8 matrix instructions with the scales in its epilogue, and the
-// straight-through gradient with respect to the input.  The reference only emulates quantised inputs and weights with dense
-// floating-point products (slim/quantization/quantization.py:219-263, :266-304).
-#include "common.hpp"
-#include "../../include/slim_hip.h"
-#include <type_traits>
+// of a weight), and the product of two such matrices on the int8 matrix instructions with the scales in its epilogue (the gradient
+// with respect to the input: int8grad.hip).  The reference only emulates quantised inputs and weights with dense floating-point
+// products (slim/quantization/quantization.py:219-263, :266-304).
+#include "int8.hpp"
 
 namespace {
 
-typedef __attribute__((ext_vector_type(4))) int i32x4;
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
-typedef const __attribute__((address_space(1))) void* glb_ptr_t;
-
-int64_t pad128(int64_t k) { return (k + 127) / 128 * 128; }
-int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
-int planes_of(int dtype) { return dtype == SLIM_DTYPE_F32 ? 3 : 2; }
-bool known(int dtype) { return dtype == SLIM_DTYPE_F32 || dtype == SLIM_DTYPE_BF16 || dtype == SLIM_DTYPE_F16; }
-int64_t element_size(int dtype) { return dtype == SLIM_DTYPE_F32 ? 4 : 2; }
-
-// ---- element types --------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(bf16_t v) { return bf16_to_f32(v); }
-__device__ __forceinline__ float to_f32(_Float16 v) { return (float)v; }
-
-// eight consecutive elements from any element-aligned address (global loads need no more than that)
-template <typename T>
-struct Packed8 {
-    typedef T vec __attribute__((ext_vector_type(8)));
-    struct __attribute__((packed, aligned(sizeof(T)))) type { vec v; };
-};
-// (ONCE: data that is not read again and need not stay in the caches)
-template <bool ONCE = false, typename T>
-__device__ __forceinline__ void load8(const T* p, int64_t valid, float out[8]) {
-    if (valid >= 8) {
-        typedef typename Packed8<T>::vec unaligned __attribute__((aligned(sizeof(T))));
-        const typename Packed8<T>::vec v = ONCE ? __builtin_nontemporal_load((const unaligned*)p) : ((const typename Packed8<T>::type*)p)->v;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) out[j] = to_f32((T)v[j]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) out[j] = j < valid ? to_f32(p[j]) : 0.f;
-    }
-}
-
 // ---- rows -> codes --------------------------------------------------------------------------------------------------
-// a = max |x| over the row, scale = a / L, q = rint(x * (L / a)) with L = 127 for one plane of codes.  PLANES > 1 (gradients):
-// the row, each element first multiplied by its column's factor, is kept as integers of more bits, q = sum 256^i * plane_i with
-// every plane in [-128, 127], so L = 127 * (256^PLANES - 1) / 255 (32639, 8355711).  Rows with a < 2^-100 become zero (scale 0); rows
-// that hold an infinity or a NaN get the scale NaN and zero codes, which makes every product with them NaN.
-// Plane rows are stored sixteen rows of plane PLANES-1 (the highest), then the sixteen of the next plane, and so on, per
-// sixteen rows of x: a fragment of the matrix product then holds all planes of its rows in one lane's accumulators.
-template <int PLANES>
-struct Levels {
-    static constexpr float value = PLANES == 1 ? 127.f : PLANES == 2 ? 32639.f : 8355711.f;
-};
-
+// a = max |x| over the row, scale = a / 127, q = rint(x * (127 / a)).  Rows with a < 2^-100 become zero (scale 0); rows that hold an
+// infinity or a NaN get the scale NaN and zero codes, which makes every product with them NaN.
 struct RowScale {
     float scale, inverse;
     bool none;                                           // nothing to keep, or nothing that could be kept
 };
-template <int PLANES>
 __device__ __forceinline__ RowScale row_scale(uint32_t max_bits) {
     const float a = __uint_as_float(max_bits);
     const bool bad = max_bits >= 0x7f800000u, none = bad || a < 0x1p-100f;
-    return {bad ? __uint_as_float(0x7fc00000u) : none ? 0.f : a / Levels<PLANES>::value, none ? 0.f : Levels<PLANES>::value / a, none};
+    return {bad ? __uint_as_float(0x7fc00000u) : none ? 0.f : a / 127.f, none ? 0.f : 127.f / a, none};
 }
 
-template <int PLANES>
-__device__ __forceinline__ void encode(const float x[8], float r, uint32_t (&out)[PLANES][2]) {
+__device__ __forceinline__ uint2 encode(const float x[8], float r) {
+    uint32_t out[2] = {0, 0};
 #pragma unroll
-    for (int p = 0; p < PLANES; ++p) out[p][0] = out[p][1] = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        float t = x[j] * r;
-        if (PLANES == 3) t = fminf(fmaxf(t, -Levels<3>::value), Levels<3>::value);    // two roundings at 23 bits can pass the last level
-        int q = (int)rintf(t);
-#pragma unroll
-        for (int p = PLANES - 1; p >= 0; --p) {          // the lowest plane first
-            const int low = p ? (int)(int8_t)(q & 255) : q;
-            out[p][j >> 2] |= (uint32_t)(low & 255) << (8 * (j & 3));
-            q = (q - low) >> 8;
-        }
-    }
-}
-template <int PLANES>
-__device__ __forceinline__ void store_codes(const float x[8], float r, int8_t* codes, int64_t ldc, int64_t row, int64_t col) {
-    uint32_t out[PLANES][2];
-    encode<PLANES>(x, r, out);
-#pragma unroll
-    for (int p = 0; p < PLANES; ++p) {
-        const int64_t at = PLANES == 1 ? row : ((row >> 4) * PLANES + p) * 16 + (row & 15);
-        *(uint2*)(codes + at * ldc + col) = make_uint2(out[p][0], out[p][1]);
-    }
+    for (int j = 0; j < 8; ++j) out[j >> 2] |= (uint32_t)((int)rintf(x[j] * r) & 255) << (8 * (j & 3));
+    return make_uint2(out[0], out[1]);
 }
 
 // WPR waves work on a row (one: four rows per workgroup; four or sixteen: one); each thread keeps NV pieces of eight elements in registers, so
 // the row is read once, with loads that do not stay in the caches (28672 x 8192 bf16: 109 us, 6.4 TB/s; 126 without).
 // NV = 0: rows too long for that are read twice.
-template <typename T, int PLANES, int NV, int WPR>
+template <typename T, int NV, int WPR>
 __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void quantize_rows_kernel(const T* __restrict__ x, int64_t R, int64_t K, int64_t ldx,
-                                                            const float* __restrict__ colscale, int8_t* __restrict__ codes,
-                                                            int64_t ldc, float* __restrict__ scale) {
+                                                            int8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scale) {
     constexpr int TPR = 64 * WPR;                        // threads of a row
     __shared__ uint32_t part[WPR];
     const int wave = threadIdx.x >> 6;
@@ -110,15 +41,7 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void quantize_rows_kernel(c
     const T* src = x + row * ldx;
     float keep[NV > 0 ? NV : 1][8];
     uint32_t m = 0;
-    auto fetch = [&](int64_t c, float v[8]) {
-        load8<(NV > 0)>(src + c, K - c, v);
-        if (PLANES > 1) {
-            float f[8];
-            load8(colscale + c, K - c, f);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= f[j];
-        }
-    };
+    auto fetch = [&](int64_t c, float v[8]) { load8<(NV > 0)>(src + c, K - c, v); };
     auto take = [&](const float v[8]) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -156,7 +79,7 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void quantize_rows_kernel(c
 #pragma unroll
         for (int i = 0; i < WPR; ++i) m = max(m, part[i]);
     }
-    const RowScale rs = row_scale<PLANES>(m);
+    const RowScale rs = row_scale(m);
     if (t == 0) scale[row] = rs.scale;
     const int64_t end = (K + 127) / 128 * 128;
     auto put = [&](int64_t c, float v[8]) {
@@ -164,7 +87,7 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void quantize_rows_kernel(c
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = 0.f;
         }
-        store_codes<PLANES>(v, rs.inverse, codes, ldc, row, c);
+        *(uint2*)(codes + row * ldc + c) = encode(v, rs.inverse);
     };
     if (NV > 0) {
 #pragma unroll
@@ -181,13 +104,12 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void quantize_rows_kernel(c
     }
 }
 
-template <typename T, int PLANES>
-int quantize_rows(const T* x, int64_t R, int64_t K, int64_t ldx, const float* colscale, int8_t* codes, int64_t ldc, float* scale,
-                  hipStream_t st) {
+template <typename T>
+int quantize_rows(const T* x, int64_t R, int64_t K, int64_t ldx, int8_t* codes, int64_t ldc, float* scale, hipStream_t st) {
     const int64_t pieces = (K + 127) / 128 * 16;         // pieces of eight codes in a padded row
     SLIM_REQUIRE(R * (pieces > 1024 ? 1024 : 256) < (int64_t)1 << 32, "quantize_rows8: too many rows for one launch");
 #define SLIM_ROWS(NV, WPR)                                                                                                  \
-    quantize_rows_kernel<T, PLANES, NV, WPR><<<(unsigned)(WPR > 1 ? R : ceil_div64(R, 4)), WPR == 16 ? 1024 : 256, 0, st>>>(x, R, K, ldx, colscale, codes, ldc, scale)
+    quantize_rows_kernel<T, NV, WPR><<<(unsigned)(WPR > 1 ? R : ceil_div64(R, 4)), WPR == 16 ? 1024 : 256, 0, st>>>(x, R, K, ldx, codes, ldc, scale)
     if (pieces <= 64) SLIM_ROWS(1, 1);
     else if (pieces <= 128) SLIM_ROWS(2, 1);
     else if (pieces <= 256) SLIM_ROWS(4, 1);
@@ -202,23 +124,21 @@ int quantize_rows(const T* x, int64_t R, int64_t K, int64_t ldx, const float* co
     return SLIM_OK;
 }
 
-template <int PLANES>
-int quantize_rows_any(const void* x, int dtype, int64_t R, int64_t K, int64_t ldx, const float* colscale, int8_t* codes, int64_t ldc,
-                      float* scale, hipStream_t st) {
-    if (dtype == SLIM_DTYPE_F32) return quantize_rows<float, PLANES>((const float*)x, R, K, ldx, colscale, codes, ldc, scale, st);
-    if (dtype == SLIM_DTYPE_BF16) return quantize_rows<bf16_t, PLANES>((const bf16_t*)x, R, K, ldx, colscale, codes, ldc, scale, st);
-    return quantize_rows<_Float16, PLANES>((const _Float16*)x, R, K, ldx, colscale, codes, ldc, scale, st);
+int quantize_rows_any(const void* x, int dtype, int64_t R, int64_t K, int64_t ldx, int8_t* codes, int64_t ldc, float* scale, hipStream_t st) {
+    if (dtype == SLIM_DTYPE_F32) return quantize_rows<float>((const float*)x, R, K, ldx, codes, ldc, scale, st);
+    if (dtype == SLIM_DTYPE_BF16) return quantize_rows<bf16_t>((const bf16_t*)x, R, K, ldx, codes, ldc, scale, st);
+    return quantize_rows<_Float16>((const _Float16*)x, R, K, ldx, codes, ldc, scale, st);
 }
 
 // ---- codes x codes --------------------------------------------------------------------------------------------------
 struct Gemm8Args {
-    const int8_t* A;                                     // [rows, lda]: rows of codes (planes interleaved when PLANES > 1)
+    const int8_t* A;                                     // [M, lda]: rows of codes
     const int8_t* B;                                     // [N, ldb]
     int64_t lda, ldb;
-    int64_t rows, M, N;                                  // rows of A, rows of the result
+    int64_t M, N;
     int steps;                                           // 128-byte steps of the reduction
     const float* sa;                                     // [M]
-    const float* sb;                                     // [N] or null
+    const float* sb;                                     // [N]
     const void* bias;                                    // [N] of the output's type, or null
     void* out;
     int64_t ldo;
@@ -228,11 +148,6 @@ struct Gemm8Args {
     int32_t* slab;                                       // [splits][tiles_m * BM][tiles_n * BN], or null: one slice, results written here
     int rest_n;                                          // columns of narrower tiles behind the tiles_n full ones (0: none)
 };
-
-template <int N>
-__device__ __forceinline__ void wait_vmcnt() {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
 
 __device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int dtype) {
     if (dtype == SLIM_DTYPE_F32) return ((const float*)p)[i];
@@ -245,69 +160,9 @@ __device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float v)
     else ((_Float16*)p)[i] = (_Float16)v;
 }
 
-// CNT (8 or 4) consecutive results of one row, to any element-aligned address
-template <int CNT, typename T, typename F>
-__device__ __forceinline__ void store_run(T* dst, int64_t left, F value) {
-    if (left >= CNT) {
-        typedef T vec __attribute__((ext_vector_type(CNT)));
-        struct __attribute__((packed, aligned(sizeof(T)))) unaligned { vec v; };
-        vec v;
-#pragma unroll
-        for (int j = 0; j < CNT; ++j) v[j] = value(j);
-        ((unaligned*)dst)->v = v;
-    } else {
-#pragma unroll
-        for (int j = 0; j < CNT; ++j)
-            if (j < left) dst[j] = value(j);
-    }
-}
-template <int CNT, typename T>
-__device__ __forceinline__ void load_run(const T* src, int64_t left, float* out) {
-    if constexpr (CNT == 8) {
-        load8(src, left, out);
-    } else {
-#pragma unroll
-        for (int c = 0; c < CNT; ++c) out[c] = c < left ? to_f32(src[c]) : 0.f;
-    }
-}
-
-// One value from its planes' sums, the highest plane first.
-template <int PLANES>
-__device__ __forceinline__ float join_planes(const int* sums, int stride) {
-    float v = (float)sums[0];
-#pragma unroll
-    for (int p = 1; p < PLANES; ++p) v = v * 256.f + (float)sums[p * stride];
-    return v;
-}
-
-// Tile and slice of workgroup b of tiles_m * tiles_n * splits.  Workgroups go to the eight XCDs in turn; each XCD gets a run of
-// consecutive tiles, and a run walks groups of eight rows of tiles column by column, so that the 32 workgroups of an XCD share 8
-// panels of A and 4 of B in its L2 (4096 x 11008 x 4096 on the 256 x 256 tile: 159 us, with groups of four 171 us).
-__device__ __forceinline__ void tile_of(int b, int tiles_m, int tiles_n, int splits, int& tm, int& tn, int& slice) {
-    const int per = tiles_m * tiles_n, total = per * splits, x = b & 7, share = total >> 3, rest = total & 7;
-    const int t = x * share + min(x, rest) + (b >> 3);
-    slice = t / per;
-    const int u = t - slice * per, group = u / (8 * tiles_n), m0 = group * 8, gm = min(8, tiles_m - m0), r = u - group * 8 * tiles_n;
-    tm = m0 + r % gm;
-    tn = r / gm;
-}
-
-// The runs of consecutive columns that a lane holds of a row of its wave's part, 4 FN values: eight per two fragments, four of an odd last one.
-// each(n0, fq, take) calls take(how many, first value, column) for each.
-template <int FN>
-struct Columns {
-    static constexpr int PAIRS = FN / 2 * 32, RUNS = (FN + 1) / 2;
-    template <typename F>
-    static __device__ __forceinline__ void each(int64_t n0, int fq, F take) {
-#pragma unroll
-        for (int c = 0; c < FN / 2; ++c) take(std::integral_constant<int, 8>(), c * 8, n0 + c * 32 + fq * 8);
-        if constexpr (FN % 2) take(std::integral_constant<int, 4>(), 4 * FN - 4, n0 + PAIRS + fq * 4);
-    }
-};
-
-// A wave's sums, planes joined, scaled, with the bias, rounded and stored: rows 16 (group0 + i) + fr of the result.
-template <int PLANES, int FM, int FN>
-__device__ __forceinline__ void write_results(const Gemm8Args& g, const i32x4 (&acc)[FM][FN], const float (&sa)[FM / PLANES], const float (&sb)[4 * FN],
+// A wave's sums, scaled, with the bias, rounded and stored: rows 16 (group0 + i) + fr of the result.
+template <int FM, int FN>
+__device__ __forceinline__ void write_results(const Gemm8Args& g, const i32x4 (&acc)[FM][FN], const float (&sa)[FM], const float (&sb)[4 * FN],
                                               int64_t group0, int64_t n0, int fr, int fq) {
     float bias[4 * FN];
 #pragma unroll
@@ -322,14 +177,11 @@ __device__ __forceinline__ void write_results(const Gemm8Args& g, const i32x4 (&
     }
     auto rows = [&](auto* out, auto convert) {
 #pragma unroll
-        for (int i = 0; i < FM / PLANES; ++i) {
+        for (int i = 0; i < FM; ++i) {
             const int64_t m = (group0 + i) * 16 + fr;
             if (m >= g.M) continue;
             auto value = [&](int c) {
-                int sums[PLANES];
-#pragma unroll
-                for (int p = 0; p < PLANES; ++p) sums[p] = acc[i * PLANES + p][c >> 2][c & 3];
-                const float v = (join_planes<PLANES>(sums, 1) * sa[i]) * sb[c];
+                const float v = ((float)acc[i][c >> 2][c & 3] * sa[i]) * sb[c];
                 return convert(g.bias ? v + bias[c] : v);
             };
             Columns<FN>::each(n0, fq, [&](auto count, int c, int64_t n) { store_run<count.value>(out + m * g.ldo + n, g.N - n, [&](int k) { return value(c + k); }); });
@@ -354,7 +206,7 @@ __device__ __forceinline__ void write_results(const Gemm8Args& g, const i32x4 (&
 // Whole 128-byte lines per row: with 64-byte steps, which would allow four stages, the requests take twice as long (171 us).
 // What bounds it: without requests the loop takes 138 us, without fragment reads as well 123 us; the matrix instructions alone hold
 // the clock at about 2.1 GHz.
-template <int PLANES, int FM, int FN, int WM, int WN, int STAGES>
+template <int FM, int FN, int WM, int WN, int STAGES>
 __device__ __forceinline__ void gemm8_tile(const Gemm8Args& g, char* lds, int64_t row0, int64_t col0, int slice) {
     constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN, NW = WM * WN;
     constexpr int PIECES = (BM + BN) / 8, PPW = (PIECES + NW - 1) / NW;     // (a last wave repeats the final piece)
@@ -362,7 +214,6 @@ __device__ __forceinline__ void gemm8_tile(const Gemm8Args& g, char* lds, int64_
     constexpr int PAIRS = FN / 2 * 32;                   // columns (rows of B) of a wave's fragments taken in pairs
     constexpr int READS = FM + FN, PRODUCTS = FM * FN;
     constexpr int PACE1 = PRODUCTS / READS > 0 ? PRODUCTS / READS : 1, PACE2 = PRODUCTS / (READS + PPW) > 0 ? PRODUCTS / (READS + PPW) : 1;
-    static_assert(FM % PLANES == 0, "a wave holds whole groups of planes");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave / WN, wc = wave % WN;
     const int fr = lane & 15, fq = lane >> 4;
@@ -384,7 +235,7 @@ __device__ __forceinline__ void gemm8_tile(const Gemm8Args& g, char* lds, int64_
             if (q * 8 < BM) {
                 const int R = q * 8 + pr;
                 base[s] = g.A + row0 * g.lda;
-                off[s] = (uint32_t)(min((int64_t)R, g.rows - 1 - row0) * g.lda) + (pc ^ (R & 7)) * 16;
+                off[s] = (uint32_t)(min((int64_t)R, g.M - 1 - row0) * g.lda) + (pc ^ (R & 7)) * 16;
             } else {
                 const int R = q * 8 - BM + pr, w = R % (16 * FN), key = w < PAIRS ? (w & 3) | (((w >> 3) & 1) << 2) : w & 7;
                 base[s] = g.B + col0 * g.ldb;
@@ -472,22 +323,20 @@ __device__ __forceinline__ void gemm8_tile(const Gemm8Args& g, char* lds, int64_
         return;
     }
     // everything the epilogue reads is requested at once (loaded row by row it costs a trip to memory per row: 4 us of a 256 x 256 tile)
-    const int64_t group0 = (row0 / 16 + wr * FM) / PLANES;
-    float sa[FM / PLANES], sb[4 * FN];
+    const int64_t group0 = row0 / 16 + wr * FM;
+    float sa[FM], sb[4 * FN];
 #pragma unroll
-    for (int i = 0; i < FM / PLANES; ++i) sa[i] = g.sa[min((group0 + i) * 16 + fr, g.M - 1)];
-#pragma unroll
-    for (int c = 0; c < 4 * FN; ++c) sb[c] = 1.f;
-    if (g.sb) Columns<FN>::each(n0, fq, [&](auto count, int c, int64_t n) { load_run<count.value>(g.sb + n, g.N - n, sb + c); });
-    write_results<PLANES, FM, FN>(g, acc, sa, sb, group0, n0, fr, fq);
+    for (int i = 0; i < FM; ++i) sa[i] = g.sa[min((group0 + i) * 16 + fr, g.M - 1)];
+    Columns<FN>::each(n0, fq, [&](auto count, int c, int64_t n) { load_run<count.value>(g.sb + n, g.N - n, sb + c); });
+    write_results<FM, FN>(g, acc, sa, sb, group0, n0, fr, fq);
 }
 
-template <int PLANES, int FM, int FN, int WM, int WN, int STAGES, int OCC>
+template <int FM, int FN, int WM, int WN, int STAGES, int OCC>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm8_kernel(const Gemm8Args g) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     int tm, tn, slice;
     tile_of(blockIdx.x, g.tiles_m, g.tiles_n, g.splits, tm, tn, slice);
-    gemm8_tile<PLANES, FM, FN, WM, WN, STAGES>(g, lds, (int64_t)tm * 16 * FM * WM, (int64_t)tn * 16 * FN * WN, slice);
+    gemm8_tile<FM, FN, WM, WN, STAGES>(g, lds, (int64_t)tm * 16 * FM * WM, (int64_t)tn * 16 * FN * WN, slice);
 }
 
 // The same product by workgroups that stay, for more tiles than CUs: each takes every gridDim.x-th tile, and the stream of requests
@@ -495,12 +344,12 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm8_kernel(const Gemm8Arg
 // stores drain under the next tile's products (a workgroup a tile: 4096 x 11008 x 4096 164 us, 159 so; 8192^3 399 and 382, 8192 x 4096 x
 // 1024 47 and 41).  REST > 0: behind the columns of full tiles lie g.rest_n columns of tiles of 16 REST WN columns, which fill the last
 // round of workgroups better.  The scales of a tile come by LDS-DMA while it is multiplied.  (g.steps >= 2)
-template <int PLANES, int FM, int FN, int WM, int WN, int REST>
+template <int FM, int FN, int WM, int WN, int REST>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm8_stream_kernel(const Gemm8Args g) {
     constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN, NW = WM * WN, STAGE_BYTES = (BM + BN) * 128;
     constexpr int ALOADS = BM / 8 / NW, LOADS = (BM + BN) / 8 / NW;      // requests of a wave and step: eight rows each, A's first
     static_assert(BM % 64 == 0 && BM % (8 * NW) == 0 && 16 * WN % (8 * NW) == 0 && BM + BN <= 64 * NW, "requests and scales are dealt out evenly");
-    constexpr int LEAST = REST && REST < FN ? REST : FN, STORES = FM / PLANES * Columns<LEAST>::RUNS, STORES32 = FM / PLANES * LEAST;     // of a whole tile, at least
+    constexpr int LEAST = REST && REST < FN ? REST : FN, STORES = FM * Columns<LEAST>::RUNS, STORES32 = FM * LEAST;     // of a whole tile, at least
     extern __shared__ __attribute__((aligned(16))) char lds[];
     float* const scales = (float*)(lds + 2 * STAGE_BYTES);              // [BM] of the rows, [BN] of the columns
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -537,7 +386,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm8_stream_kernel(const Gem
         for (int s = 0; s < LOADS; ++s) {
             const int R = (s * NW + wave) * 8 + pr;
             if (s < ALOADS) {
-                off[s] = (uint32_t)(min((int64_t)R, g.rows - 1 - row0) * g.lda) + (pc ^ (R & 7)) * 16;
+                off[s] = (uint32_t)(min((int64_t)R, g.M - 1 - row0) * g.lda) + (pc ^ (R & 7)) * 16;
             } else {
                 const int r = R - BM, w = narrow ? r % (16 * (REST ? REST : 1)) : r % (16 * FN), pairs = narrow ? Columns<REST>::PAIRS : Columns<FN>::PAIRS;
                 const int key = w < pairs ? (w & 3) | (((w >> 3) & 1) << 2) : w & 7;
@@ -619,8 +468,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm8_stream_kernel(const Gem
                 asm volatile("" ::: "memory");
                 if (kt == 0) {                           // every wave is past the tile before: this one's scales, for its end
                     const int t = wave * 64 + this_lane();
-                    const float* src = wave * 64 < BM ? g.sa + min(row0 / PLANES + t, g.M - 1) : g.sb + min(col0 + t - BM, g.N - 1);
-                    if (wave * 64 < BM || (g.sb && wave * 64 < BM + BN)) __builtin_amdgcn_global_load_lds((glb_ptr_t)src, (lds_ptr_t)(scales + wave * 64), 4, 0, 0);
+                    const float* src = wave * 64 < BM ? g.sa + min(row0 + t, g.M - 1) : g.sb + min(col0 + t - BM, g.N - 1);
+                    if (wave * 64 < BM + BN) __builtin_amdgcn_global_load_lds((glb_ptr_t)src, (lds_ptr_t)(scales + wave * 64), 4, 0, 0);
                 }
                 __builtin_amdgcn_sched_barrier(0);
                 read(0, stage ^ 1);
@@ -641,20 +490,17 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm8_stream_kernel(const Gem
             }
             asm volatile("" ::: "memory");               // (no store moves in front of the requests)
             const int l = this_lane(), er = l & 15, eq = l >> 4;
-            float sa[FM / PLANES], sb[4 * F];
+            float sa[FM], sb[4 * F];
 #pragma unroll
-            for (int i = 0; i < FM / PLANES; ++i) sa[i] = scales[(wr * FM / PLANES + i) * 16 + er];
-#pragma unroll
-            for (int c = 0; c < 4 * F; ++c) sb[c] = 1.f;
+            for (int i = 0; i < FM; ++i) sa[i] = scales[(wr * FM + i) * 16 + er];
             const int64_t n0 = col0 + wc * 16 * F;
-            if (g.sb)
-                Columns<F>::each(n0, eq, [&](auto count, int c, int64_t n) {
+            Columns<F>::each(n0, eq, [&](auto count, int c, int64_t n) {
 #pragma unroll
-                    for (int j = 0; j < count.value; ++j) sb[c + j] = scales[BM + (int)(n - col0) + j];
-                });
-            write_results<PLANES, FM, F>(g, acc, sa, sb, (row0 / 16 + wr * FM) / PLANES, n0, er, eq);
+                for (int j = 0; j < count.value; ++j) sb[c + j] = scales[BM + (int)(n - col0) + j];
+            });
+            write_results<FM, F>(g, acc, sa, sb, row0 / 16 + wr * FM, n0, er, eq);
             asm volatile("" ::: "memory");
-            stores = row0 / PLANES + BM / PLANES <= g.M && col0 + 16 * F * WN <= g.N;
+            stores = row0 + BM <= g.M && col0 + 16 * F * WN <= g.N;
         }
     };
     tiles(std::integral_constant<int, FN>(), full);
@@ -662,27 +508,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void gemm8_stream_kernel(const Gem
     wait_vmcnt<0>();                                     // (the requests behind the last step land before the LDS is given up)
 }
 
-// The slices' sums added (whole numbers: any order gives the same), planes joined, scaled and rounded: a thread per four columns.
-template <int PLANES>
+// The slices' sums added (whole numbers: any order gives the same), scaled and rounded: a thread per four columns.
 __global__ __launch_bounds__(256) void join_slices_kernel(const Gemm8Args g, int64_t slab_rows, int64_t slab_cols) {
     const int64_t quads = (g.N + 3) / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t m = i / quads, n = (i - m * quads) * 4;
     if (m >= g.M) return;
-    i32x4 sum[PLANES];
-#pragma unroll
-    for (int p = 0; p < PLANES; ++p) sum[p] = i32x4{0, 0, 0, 0};
-    const int32_t* src = g.slab + ((m / 16) * 16 * PLANES + m % 16) * slab_cols + n;
-    for (int z = 0; z < g.splits; ++z, src += slab_rows * slab_cols)
-#pragma unroll
-        for (int p = 0; p < PLANES; ++p) sum[p] += *(const i32x4*)(src + p * 16 * slab_cols);
+    i32x4 sum = i32x4{0, 0, 0, 0};
+    const int32_t* src = g.slab + m * slab_cols + n;
+    for (int z = 0; z < g.splits; ++z, src += slab_rows * slab_cols) sum += *(const i32x4*)src;
     const float sa = g.sa[m];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         if (n + c >= g.N) break;
-        int sums[PLANES];
-#pragma unroll
-        for (int p = 0; p < PLANES; ++p) sums[p] = sum[p][c];
-        float v = (join_planes<PLANES>(sums, 1) * sa) * (g.sb ? g.sb[n + c] : 1.f);
+        float v = ((float)sum[c] * sa) * g.sb[n + c];
         if (g.bias) v += load_as_f32(g.bias, n + c, g.dtype);
         store_as(g.out, m * g.ldo + n + c, g.dtype, v);
     }
@@ -698,18 +536,10 @@ struct Tile {
     int bm, bn, places;                                  // workgroups that share a CU
     double ends, alone, full;
 };
-template <int PLANES>
-struct Tiles {
-    static constexpr int count = 5;
-    static constexpr Tile list[5] = {{256, 256, 1, 7.0, 1.02, 1.60}, {128, 256, 1, 5.0, 0.60, 0.97}, {128, 128, 1, 4.3, 0.34, 0.53},
-                                     {64, 128, 1, 3.6, 0.24, 0.345},     // four stages, a CU for each workgroup ...
-                                     {64, 128, 2, 3.4, 0.34, 0.65}};     // ... or three and two workgroups a CU
-};
-template <>
-struct Tiles<3> {                                        // (a wave's rows are a multiple of 48)
-    static constexpr int count = 2;
-    static constexpr Tile list[2] = {{192, 256, 1, 6.0, 0.80, 1.25}, {96, 128, 1, 4.0, 0.35, 0.50}};
-};
+constexpr int TILES = 5;
+constexpr Tile tiles[TILES] = {{256, 256, 1, 7.0, 1.02, 1.60}, {128, 256, 1, 5.0, 0.60, 0.97}, {128, 128, 1, 4.3, 0.34, 0.53},
+                               {64, 128, 1, 3.6, 0.24, 0.345},     // four stages, a CU for each workgroup ...
+                               {64, 128, 2, 3.4, 0.34, 0.65}};     // ... or three and two workgroups a CU
 struct Plan {
     int tile = 0, splits = 1, steps_per_split = 0;
     int64_t tiles_m = 0, tiles_n = 0, slab_rows = 0, slab_cols = 0;
@@ -718,22 +548,21 @@ struct Plan {
     bool stays() const { return tile == 0 && splits == 1 && steps_per_split >= 2 && tiles_m * (tiles_n + rest_n) > 256; }     // workgroups take several tiles
     int64_t slab_bytes() const { return splits > 1 ? splits * slab_rows * slab_cols * 4 : 0; }
 };
-template <int PLANES>
-Plan plan_gemm8(int64_t rows, int64_t N, int64_t steps) {
+Plan plan_gemm8(int64_t M, int64_t N, int64_t steps) {
     Plan best;
     double best_time = 1e30;
-    for (int k = 0; k < Tiles<PLANES>::count; ++k) {
-        const Tile t = Tiles<PLANES>::list[k];
-        const int64_t tiles_m = ceil_div64(rows, t.bm), tiles_n = ceil_div64(N, t.bn), tiles = tiles_m * tiles_n;
-        for (int splits = 1; splits <= 8 && (splits == 1 || (steps >= 8 * splits && tiles * splits <= 256)); splits *= 2) {
-            const int64_t each = ceil_div64(steps, splits), groups = tiles * splits, slots = 256 * t.places;
+    for (int k = 0; k < TILES; ++k) {
+        const Tile t = tiles[k];
+        const int64_t tiles_m = ceil_div64(M, t.bm), tiles_n = ceil_div64(N, t.bn), count = tiles_m * tiles_n;
+        for (int splits = 1; splits <= 8 && (splits == 1 || (steps >= 8 * splits && count * splits <= 256)); splits *= 2) {
+            const int64_t each = ceil_div64(steps, splits), groups = count * splits, slots = 256 * t.places;
             const int64_t rest = groups % slots;
             auto round = [&](int64_t n) {                // n workgroups, at most `slots`
                 const double busy = t.places == 2 ? (n > 256 ? 1.0 : 0.0) : n / 256.0;
                 return t.ends + each * (t.alone + (t.full - t.alone) * busy);
             };
             double time = (groups / slots) * round(slots) + (rest ? round(rest) : 0.0);
-            if (splits > 1) time += 3.0 + 2.0 * splits * tiles * t.bm * t.bn * 4 / 4e6;
+            if (splits > 1) time += 3.0 + 2.0 * splits * count * t.bm * t.bn * 4 / 4e6;
             if (time < best_time) {
                 best_time = time;
                 best.tile = k, best.splits = (int)ceil_div64(steps, each), best.steps_per_split = (int)each;
@@ -743,12 +572,12 @@ Plan plan_gemm8(int64_t rows, int64_t N, int64_t steps) {
     }
     // The largest tile's last round, when it is not full, on narrower tiles that fill it better (4096 x 11008: 512 full tiles and 240 of
     // 192 columns in place of 176 full ones).
-    if (PLANES < 3 && best.tile == 0 && best.splits == 1 && best.steps_per_split >= 2 && best.tiles_m <= 256) {
-        const int64_t tiles = best.tiles_m * best.tiles_n, columns = tiles / 256 * 256 / best.tiles_m;
-        if (tiles > 256 && tiles % 256 && columns < best.tiles_n) {
+    if (best.tile == 0 && best.splits == 1 && best.steps_per_split >= 2 && best.tiles_m <= 256) {
+        const int64_t count = best.tiles_m * best.tiles_n, columns = count / 256 * 256 / best.tiles_m;
+        if (count > 256 && count % 256 && columns < best.tiles_n) {
             for (int rest = 3; rest >= 2; --rest) {
                 const int64_t n = ceil_div64(N - columns * 256, 64 * rest);
-                if (columns * best.tiles_m + n * best.tiles_m <= (tiles / 256 + 1) * 256) best.rest = rest, best.rest_n = n;
+                if (columns * best.tiles_m + n * best.tiles_m <= (count / 256 + 1) * 256) best.rest = rest, best.rest_n = n;
             }
             if (best.rest) best.tiles_n = columns;
         }
@@ -756,55 +585,49 @@ Plan plan_gemm8(int64_t rows, int64_t N, int64_t steps) {
     return best;
 }
 
-template <int PLANES, int TILE, int FM, int FN, int WM, int WN, int STAGES, int OCC>
+template <int TILE, int FM, int FN, int WM, int WN, int STAGES, int OCC>
 int launch_gemm8(const Gemm8Args& g, const Plan& p, hipStream_t st) {
     constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN, bytes = STAGES * (BM + BN) * 128;
     const int64_t blocks = p.tiles_m * p.tiles_n * p.splits;
-    static_assert(Tiles<PLANES>::list[TILE].bm == BM && Tiles<PLANES>::list[TILE].bn == BN, "the plan's tile");
+    static_assert(tiles[TILE].bm == BM && tiles[TILE].bn == BN, "the plan's tile");
     SLIM_REQUIRE(blocks * 64 * WM * WN < (int64_t)1 << 32 && blocks < 0x7fffffff, "gemm8: the result is too large for one launch");
-    auto kernel = gemm8_kernel<PLANES, FM, FN, WM, WN, STAGES, OCC>;
+    auto kernel = gemm8_kernel<FM, FN, WM, WN, STAGES, OCC>;
     SLIM_HIP(slim_allow_dynamic_lds((const void*)kernel, bytes));
     kernel<<<(unsigned)blocks, 64 * WM * WN, bytes, st>>>(g);
     SLIM_LAUNCH_CHECK();
     return SLIM_OK;
 }
 
-template <int PLANES, int FM, int REST>
+template <int REST>
 int launch_stream8(const Gemm8Args& g, const Plan& p, hipStream_t st) {
-    constexpr int bytes = (32 * FM + 256) * (2 * 128 + 4);
-    static_assert(Tiles<PLANES>::list[0].bm == 32 * FM && Tiles<PLANES>::list[0].bn == 256, "the plan's tile");
+    constexpr int bytes = (256 + 256) * (2 * 128 + 4);
+    static_assert(tiles[0].bm == 256 && tiles[0].bn == 256, "the plan's tile");
     SLIM_REQUIRE(p.tiles_m * (p.tiles_n + p.rest_n) < 0x7fffffff - 256, "gemm8: the result is too large for one launch");
-    auto kernel = gemm8_stream_kernel<PLANES, FM, 4, 2, 4, REST>;
+    auto kernel = gemm8_stream_kernel<8, 4, 2, 4, REST>;
     SLIM_HIP(slim_allow_dynamic_lds((const void*)kernel, bytes));
     kernel<<<256, 512, bytes, st>>>(g);
     SLIM_LAUNCH_CHECK();
     return SLIM_OK;
 }
 
-template <int PLANES>
 int gemm8(Gemm8Args g, void* slab, hipStream_t st) {
-    SLIM_PROF("gemm8", st, (double)g.rows * g.steps * 128 + (double)g.N * g.steps * 128 + (double)g.M * g.N * element_size(g.dtype),
-              2.0 * g.rows * g.N * g.steps * 128);
-    const Plan p = plan_gemm8<PLANES>(g.rows, g.N, g.steps);
+    SLIM_PROF("gemm8", st, (double)(g.M + g.N) * g.steps * 128 + (double)g.M * g.N * element_size(g.dtype), 2.0 * g.M * g.N * g.steps * 128);
+    const Plan p = plan_gemm8(g.M, g.N, g.steps);
     g.tiles_m = (int)p.tiles_m, g.tiles_n = (int)p.tiles_n;
     g.splits = p.splits, g.steps_per_split = p.steps_per_split, g.rest_n = (int)p.rest_n;
     g.slab = p.splits > 1 ? (int32_t*)slab : nullptr;
     int rc;
-    if constexpr (PLANES == 3) {
-        rc = p.stays() ? launch_stream8<3, 6, 0>(g, p, st) : p.tile == 0 ? launch_gemm8<3, 0, 6, 4, 2, 4, 2, 2>(g, p, st) : launch_gemm8<3, 1, 3, 2, 2, 4, 4, 2>(g, p, st);
-    } else {
-        if (p.stays() && p.rest == 3) rc = launch_stream8<PLANES, 8, 3>(g, p, st);
-        else if (p.stays() && p.rest == 2) rc = launch_stream8<PLANES, 8, 2>(g, p, st);
-        else if (p.stays()) rc = launch_stream8<PLANES, 8, 0>(g, p, st);
-        else if (p.tile == 0) rc = launch_gemm8<PLANES, 0, 8, 4, 2, 4, 2, 2>(g, p, st);
-        else if (p.tile == 1) rc = launch_gemm8<PLANES, 1, 4, 4, 2, 4, 3, 2>(g, p, st);
-        else if (p.tile == 2) rc = launch_gemm8<PLANES, 2, 4, 2, 2, 4, 4, 2>(g, p, st);
-        else if (p.tile == 3) rc = launch_gemm8<PLANES, 3, 2, 2, 2, 4, 4, 2>(g, p, st);
-        else rc = launch_gemm8<PLANES, 4, 2, 2, 2, 4, 3, 4>(g, p, st);
-    }
+    if (p.stays() && p.rest == 3) rc = launch_stream8<3>(g, p, st);
+    else if (p.stays() && p.rest == 2) rc = launch_stream8<2>(g, p, st);
+    else if (p.stays()) rc = launch_stream8<0>(g, p, st);
+    else if (p.tile == 0) rc = launch_gemm8<0, 8, 4, 2, 4, 2, 2>(g, p, st);
+    else if (p.tile == 1) rc = launch_gemm8<1, 4, 4, 2, 4, 3, 2>(g, p, st);
+    else if (p.tile == 2) rc = launch_gemm8<2, 4, 2, 2, 4, 4, 2>(g, p, st);
+    else if (p.tile == 3) rc = launch_gemm8<3, 2, 2, 2, 4, 4, 2>(g, p, st);
+    else rc = launch_gemm8<4, 2, 2, 2, 4, 3, 4>(g, p, st);
     if (rc || p.splits == 1) return rc;
     const int64_t threads = g.M * ((g.N + 3) / 4);
-    join_slices_kernel<PLANES><<<(unsigned)ceil_div64(threads, 256), 256, 0, st>>>(g, p.slab_rows, p.slab_cols);
+    join_slices_kernel<<<(unsigned)ceil_div64(threads, 256), 256, 0, st>>>(g, p.slab_rows, p.slab_cols);
     SLIM_LAUNCH_CHECK();
     return SLIM_OK;
 }
@@ -816,12 +639,12 @@ int gemm8(Gemm8Args g, void* slab, hipStream_t st) {
 // barrier is that in front of the sums' addition.  (Loaded straight into the matrix instructions' layout, 16 rows by 64 bytes a
 // request, the weight takes half as long again.)
 struct RingArgs {
-    const int8_t* A;                                     // codes of the tokens (planes interleaved when PLANES > 1)
-    int64_t lda, rows;
+    const int8_t* A;                                     // codes of the tokens
+    int64_t lda;
     const float* sa;
     const int8_t* B;
     int64_t ldb;
-    const float* sb;                                     // or null
+    const float* sb;
     const void* bias;
     void* out;
     int64_t ldo;
@@ -831,39 +654,35 @@ struct RingArgs {
 };
 // The waves' sums, `stride` bytes from one wave's to the next, added: a result per thread and turn, channel n of token m (the
 // instruction's rows are channels, its columns tokens).  sa: the scales of the workgroup's tokens.
-template <int PLANES, int FM, int FN, int NW>
+template <int FM, int FN, int NW>
 __device__ __forceinline__ void wave_results(const RingArgs& g, const char* sums, int stride, const float* sa, int64_t m0, int64_t n0) {
-    for (int t = threadIdx.x; t < 256 * FM / PLANES * FN; t += 64 * NW) {
+    for (int t = threadIdx.x; t < 256 * FM * FN; t += 64 * NW) {
         const int n = t % (16 * FN), m = t / (16 * FN);
         if (m0 + m >= g.M || n0 + n >= g.N) continue;
-        int sum[PLANES];
+        const int at = ((m >> 4) * FN + (n >> 4)) * 64 + ((n & 15) >> 2) * 16 + (m & 15);
+        int sum = 0;
 #pragma unroll
-        for (int p = 0; p < PLANES; ++p) {
-            const int at = (((m >> 4) * PLANES + p) * FN + (n >> 4)) * 64 + ((n & 15) >> 2) * 16 + (m & 15);
-            sum[p] = 0;
-#pragma unroll
-            for (int w = 0; w < NW; ++w) sum[p] += ((const int*)(sums + w * stride))[at * 4 + (n & 3)];
-        }
-        float v = (join_planes<PLANES>(sum, 1) * sa[m]) * (g.sb ? g.sb[n0 + n] : 1.f);
+        for (int w = 0; w < NW; ++w) sum += ((const int*)(sums + w * stride))[at * 4 + (n & 3)];
+        float v = ((float)sum * sa[m]) * g.sb[n0 + n];
         if (g.bias) v += load_as_f32(g.bias, n0 + n, g.dtype);
         store_as(g.out, (m0 + m) * g.ldo + n0 + n, g.dtype, v);
     }
 }
-template <int PLANES, int FM, int FN, int NW, int STAGES>
+template <int FM, int FN, int NW, int STAGES>
 __global__ __launch_bounds__(64 * NW) void ring8_kernel(const RingArgs g) {
     constexpr int REQ = 2 * FM + 2 * FN, UNIT = REQ * 1024;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
-    const int64_t n0 = (int64_t)blockIdx.x * 16 * FN, r0 = (int64_t)blockIdx.y * 16 * FM, m0 = r0 / PLANES;
+    const int64_t n0 = (int64_t)blockIdx.x * 16 * FN, m0 = (int64_t)blockIdx.y * 16 * FM;
     char* const ring = lds + wave * STAGES * UNIT;
     uint32_t off[REQ];                                   // a request: eight rows, lane / 8, of which it takes piece (lane % 8) ^ row
     {
         const int pr = lane >> 3, pc = (lane & 7) ^ pr;
 #pragma unroll
         for (int s = 0; s < REQ; ++s)
-            off[s] = (s < 2 * FM ? (uint32_t)(min((int64_t)s * 8 + pr, g.rows - 1 - r0) * g.lda) : (uint32_t)(min((int64_t)(s - 2 * FM) * 8 + pr, g.N - 1 - n0) * g.ldb)) + pc * 16;
+            off[s] = (s < 2 * FM ? (uint32_t)(min((int64_t)s * 8 + pr, g.M - 1 - m0) * g.lda) : (uint32_t)(min((int64_t)(s - 2 * FM) * 8 + pr, g.N - 1 - n0) * g.ldb)) + pc * 16;
     }
-    const int8_t *const a0 = g.A + r0 * g.lda, *const b0 = g.B + n0 * g.ldb;
+    const int8_t *const a0 = g.A + m0 * g.lda, *const b0 = g.B + n0 * g.ldb;
     const int mine = wave < g.units ? (g.units - wave + NW - 1) / NW : 0;
     auto request = [&](int i, int stage) {
         const int64_t k = (int64_t)(wave + i * NW) * 128;
@@ -911,16 +730,15 @@ __global__ __launch_bounds__(64 * NW) void ring8_kernel(const RingArgs g) {
 #pragma unroll
         for (int j = 0; j < FN; ++j) sums[(i * FN + j) * 64 + lane] = acc[i][j];
     __syncthreads();
-    wave_results<PLANES, FM, FN, NW>(g, lds, STAGES * UNIT, g.sa + m0, m0, n0);
+    wave_results<FM, FN, NW>(g, lds, STAGES * UNIT, g.sa + m0, m0, n0);
 }
 
-template <int PLANES, int FM, int FN, int NW, int STAGES>
+template <int FM, int FN, int NW, int STAGES>
 int launch_ring8_as(const RingArgs& g, hipStream_t st) {
     constexpr int bytes = NW * STAGES * (FM + FN) * 2048;
-    static_assert(FM % PLANES == 0, "a workgroup holds whole groups of planes");
-    auto kernel = ring8_kernel<PLANES, FM, FN, NW, STAGES>;
+    auto kernel = ring8_kernel<FM, FN, NW, STAGES>;
     SLIM_HIP(slim_allow_dynamic_lds((const void*)kernel, bytes));
-    kernel<<<dim3((unsigned)ceil_div64(g.N, 16 * FN), (unsigned)ceil_div64(g.rows, 16 * FM)), 64 * NW, bytes, st>>>(g);
+    kernel<<<dim3((unsigned)ceil_div64(g.N, 16 * FN), (unsigned)ceil_div64(g.M, 16 * FM)), 64 * NW, bytes, st>>>(g);
     SLIM_LAUNCH_CHECK();
     return SLIM_OK;
 }
@@ -928,50 +746,37 @@ int launch_ring8_as(const RingArgs& g, hipStream_t st) {
 // channels and eight waves 7.0, 13.8 and 21.5 for 16 tokens, 32 channels and four waves 8.0, 11.5 and 18.0; 8.2, 15.8 and 24.3 against
 // 8.9, 13.5 and 19.2 for 32.  From 33 to 64 all rows in one workgroup and eight waves where two to a CU would fill the chip (40 x 4096
 // x 11008: 12.8 against 15.4; but 64 x 1024 x 1024 3.7 against 3.2).
-// Small results of more rows, and the planes of gradients, go the same way while every workgroup finds a place at once: four waves
-// share a reduction that a tile walks step by step (rows x channels x reduction, us, tile / here: 128 x 512 x 2048 7.5 / 3.6, 512 x
-// 512 x 8192 14.6 / 11.8; gradients with their quantisation: 16 x 4096 x 4096 fp32 15.8 / 10.4, 64 x 1024 x 2048 bf16 11.7 / 7.7).  First in
-// workgroups of 32 rows of codes by sixteen channels (planes: sixteen rows of the result), two a CU, then in four times that, one a CU
-// (128 x 4096 x 2048 7.6 / 6.4, gradient 256 x 1024 x 2048 bf16 12.6 / 11.2); with more of them the tiles win (512 workgroups of the
-// second: 1024 x 1024 x 2048 8.1 / 11.5).
-template <int PLANES>
+// Small results of more rows go the same way while every workgroup finds a place at once: four waves share a reduction that a tile
+// walks step by step (rows x channels x reduction, us, tile / here: 128 x 512 x 2048 7.5 / 3.6, 512 x 512 x 8192 14.6 / 11.8).  First in
+// workgroups of 32 rows by sixteen channels, two a CU, then in four times that, one a CU (128 x 4096 x 2048 7.6 / 6.4); with more of them
+// the tiles win (512 workgroups of the second: 1024 x 1024 x 2048 8.1 / 11.5).
 int takes_ring(int64_t M, int64_t N) {                   // 0: no; 1, 2: the smaller or the larger workgroups
-    constexpr int rows = PLANES == 1 ? 32 : 16;
-    if (PLANES == 1 && M <= 32) return 1;
-    return ceil_div64(M, rows) * ceil_div64(N, 16) <= 512 ? 1 : ceil_div64(M, 2 * rows) * ceil_div64(N, 32) <= 256 ? 2 : 0;
+    if (M <= 32) return 1;
+    return ceil_div64(M, 32) * ceil_div64(N, 16) <= 512 ? 1 : ceil_div64(M, 64) * ceil_div64(N, 32) <= 256 ? 2 : 0;
 }
-template <int PLANES>
 int launch_ring8(const RingArgs& g, hipStream_t st) {
-    SLIM_PROF("ring8", st, (double)(g.N + g.rows) * g.units * 128 + (double)g.M * g.N * element_size(g.dtype), 2.0 * g.rows * g.N * g.units * 128);
-    const bool large = takes_ring<PLANES>(g.M, g.N) == 2;
-    if constexpr (PLANES == 3) {
-        return large ? launch_ring8_as<3, 6, 2, 4, 2>(g, st) : launch_ring8_as<3, 3, 1, 4, 2>(g, st);
-    } else if constexpr (PLANES == 2) {
-        return large ? launch_ring8_as<2, 4, 2, 4, 3>(g, st) : launch_ring8_as<2, 2, 1, 4, 3>(g, st);
-    } else {
-        const bool narrow = g.N <= 4096;
-        if (g.M <= 16) return narrow ? launch_ring8_as<1, 1, 1, 8, 3>(g, st) : launch_ring8_as<1, 1, 2, 4, 3>(g, st);
-        if (g.M <= 32) return narrow ? launch_ring8_as<1, 2, 1, 8, 2>(g, st) : launch_ring8_as<1, 2, 2, 4, 2>(g, st);
-        if (g.M <= 64 && narrow && g.N > 2048) return launch_ring8_as<1, 4, 1, 8, 2>(g, st);
-        return large ? launch_ring8_as<1, 4, 2, 4, 3>(g, st) : launch_ring8_as<1, 2, 1, 4, 3>(g, st);
-    }
+    SLIM_PROF("ring8", st, (double)(g.N + g.M) * g.units * 128 + (double)g.M * g.N * element_size(g.dtype), 2.0 * g.M * g.N * g.units * 128);
+    const bool narrow = g.N <= 4096;
+    if (g.M <= 16) return narrow ? launch_ring8_as<1, 1, 8, 3>(g, st) : launch_ring8_as<1, 2, 4, 3>(g, st);
+    if (g.M <= 32) return narrow ? launch_ring8_as<2, 1, 8, 2>(g, st) : launch_ring8_as<2, 2, 4, 2>(g, st);
+    if (g.M <= 64 && narrow && g.N > 2048) return launch_ring8_as<4, 1, 8, 2>(g, st);
+    return takes_ring(g.M, g.N) == 2 ? launch_ring8_as<4, 2, 4, 3>(g, st) : launch_ring8_as<2, 1, 4, 3>(g, st);
 }
 
 // ---- small products in one launch -----------------------------------------------------------------------------------
 // Sixteen rows by sixteen channels a workgroup, which quantises its rows itself (as quantize_rows_kernel does, to the same codes), two
 // rows a wave, while the weight's rows, all units at once, travel by LDS-DMA.  N / 16 workgroups repeat that: over a short reduction it
 // takes no longer than the kernel it replaces, and saves a launch and the workspace (us on the GPU, then per call from Python, two launches /
-// one: 64 x 480 x 480 5.6 / 3.9, 12.2 / 7.8; gradient of 64 x 480 x 480 bf16 5.4 / 4.5, 12.2 / 7.8).  Four waves and four rows each: 5.1 and 5.8.
-// x: [M, K], colscale: null or a factor per column (gradients).
+// one: 64 x 480 x 480 5.6 / 3.9, 12.2 / 7.8).  Four waves and four rows each: 5.1.
 constexpr int SMALL_WAVES = 8;
-template <typename T, int PLANES, int NP>
-__global__ __launch_bounds__(64 * SMALL_WAVES) void small8_kernel(const RingArgs g, const T* __restrict__ x, int64_t ldx, int K, const float* __restrict__ colscale) {
+template <typename T, int NP>
+__global__ __launch_bounds__(64 * SMALL_WAVES) void small8_kernel(const RingArgs g, const T* __restrict__ x, int64_t ldx, int K) {
     constexpr int NW = SMALL_WAVES, EACH = 16 / NW;      // rows of a wave
     extern __shared__ __attribute__((aligned(16))) char lds[];
     __shared__ float sa[16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fq = lane >> 4;
     const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * 16;
-    char* const weight = lds + g.units * PLANES * 2048;
+    char* const weight = lds + g.units * 2048;
     {
         const int pr = lane >> 3, pc = (lane & 7) ^ pr;
         const int8_t* const b0 = g.B + n0 * g.ldb;
@@ -980,21 +785,18 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void small8_kernel(const RingArgs
             for (int s = 0; s < 2; ++s)
                 __builtin_amdgcn_global_load_lds((glb_ptr_t)(b0 + u * 128 + (uint32_t)(min((int64_t)s * 8 + pr, g.N - 1 - n0) * g.ldb) + pc * 16), (lds_ptr_t)(weight + u * 2048 + s * 1024), 16, 0, 0);
     }
-    float v[EACH][NP][8], f[NP][8];
+    float v[EACH][NP][8];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int c = (i * 64 + lane) * 8;
         if (c < K) {
-            if (PLANES > 1) load8(colscale + c, (int64_t)K - c, f[i]);
 #pragma unroll
             for (int r = 0; r < EACH; ++r) load8(x + min(m0 + wave * EACH + r, g.M - 1) * ldx + c, (int64_t)K - c, v[r][i]);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                f[i][j] = 0.f;
+            for (int j = 0; j < 8; ++j)
 #pragma unroll
                 for (int r = 0; r < EACH; ++r) v[r][i][j] = 0.f;
-            }
         }
     }
 #pragma unroll
@@ -1004,13 +806,10 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void small8_kernel(const RingArgs
 #pragma unroll
         for (int i = 0; i < NP; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (PLANES > 1) v[r][i][j] *= f[i][j];
-                top = max(top, f32_bits(v[r][i][j]) & 0x7fffffffu);
-            }
+            for (int j = 0; j < 8; ++j) top = max(top, f32_bits(v[r][i][j]) & 0x7fffffffu);
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-        const RowScale rs = row_scale<PLANES>(top);
+        const RowScale rs = row_scale(top);
         if (lane == 0) sa[row] = rs.scale;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
@@ -1020,50 +819,39 @@ __global__ __launch_bounds__(64 * SMALL_WAVES) void small8_kernel(const RingArgs
 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[r][i][j] = 0.f;
             }
-            uint32_t out[PLANES][2];
-            encode<PLANES>(v[r][i], rs.inverse, out);
-            char* const dst = lds + (c >> 7) * PLANES * 2048 + row * 128 + ((((c >> 4) & 7) ^ (row & 7)) * 16) + (c & 8);
-#pragma unroll
-            for (int p = 0; p < PLANES; ++p) *(uint2*)(dst + p * 2048) = make_uint2(out[p][0], out[p][1]);
+            *(uint2*)(lds + (c >> 7) * 2048 + row * 128 + ((((c >> 4) & 7) ^ (row & 7)) * 16) + (c & 8)) = encode(v[r][i], rs.inverse);
         }
     }
     wait_vmcnt<0>();                                     // this wave's units of the weight
     __syncthreads();
-    i32x4 acc[PLANES];
-#pragma unroll
-    for (int i = 0; i < PLANES; ++i) acc[i] = i32x4{0, 0, 0, 0};
+    i32x4 acc = i32x4{0, 0, 0, 0};
     const int x0 = fr * 128 + (fq ^ (fr & 7)) * 16;
     for (int u = wave; u < g.units; u += NW)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const i32x4 b = *(const i32x4*)(weight + u * 2048 + (x0 ^ (h * 64)));
-#pragma unroll
-            for (int i = 0; i < PLANES; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, *(const i32x4*)(lds + (u * PLANES + i) * 2048 + (x0 ^ (h * 64))), acc[i], 0, 0, 0);
+            const i32x4 a = *(const i32x4*)(lds + u * 2048 + (x0 ^ (h * 64))), b = *(const i32x4*)(weight + u * 2048 + (x0 ^ (h * 64)));
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, a, acc, 0, 0, 0);
         }
     __syncthreads();                                     // (no one reads the codes any more)
-#pragma unroll
-    for (int i = 0; i < PLANES; ++i) ((i32x4*)lds)[(wave * PLANES + i) * 64 + lane] = acc[i];
+    ((i32x4*)lds)[wave * 64 + lane] = acc;
     __syncthreads();
-    wave_results<PLANES, PLANES, 1, NW>(g, lds, PLANES * 1024, sa, m0, n0);
+    wave_results<1, 1, NW>(g, lds, 1024, sa, m0, n0);
 }
 // How many workgroups may repeat a reduction of one, two or four pieces of 512 (us on the GPU, two launches / one: 512 x 512 x 512 6.2 / 6.2,
 // 3000 x 100 x 500 9.9 / 9.0 - 10.7; 64 x 2048 x 1000 6.1 / 5.8, 256 x 1024 x 1024 7.0 / 8.5; 64 x 480 x 2048 7.2 / 5.9, 128 x 1024 x 2048 7.4 /
-// 8.6; gradients: 256 x 500 x 1000 bf16 7.3 / 7.2, 500 x 512 x 200 fp32 7.9 / 8.9, 64 x 2048 x 1000 fp32 7.1 / 8.7, 77 x 776 x 1000 6.5 / 6.6,
-// 16 x 512 x 2048 7.6 / 8.5).
-template <int PLANES>
+// 8.6).
 bool takes_small(int64_t M, int64_t N, int64_t K) {
-    if (K > (PLANES == 1 ? 2048 : 1024)) return false;
-    const int64_t pieces = K <= 512 ? 1 : K <= 1024 ? 2 : 4, most = PLANES == 1 ? 1024 / pieces : PLANES == 2 ? 512 : 512 / pieces;
-    return ceil_div64(M, 16) * ceil_div64(N, 16) <= most;
+    if (K > 2048) return false;
+    const int64_t pieces = K <= 512 ? 1 : K <= 1024 ? 2 : 4;
+    return ceil_div64(M, 16) * ceil_div64(N, 16) <= 1024 / pieces;
 }
-template <typename T, int PLANES>
-int launch_small8(const RingArgs& g, const T* x, int64_t ldx, int64_t K, const float* colscale, hipStream_t st) {
-    SLIM_PROF("small8", st, (double)g.M * K * sizeof(T) + (double)g.N * g.units * 128 + (double)g.M * g.N * sizeof(T), 2.0 * PLANES * g.M * g.N * K);
-    auto kernel = K <= 512 ? small8_kernel<T, PLANES, 1> : small8_kernel<T, PLANES, 2>;
-    if constexpr (PLANES == 1) kernel = K <= 1024 ? kernel : small8_kernel<T, 1, 4>;
-    const int bytes = max(g.units * (PLANES + 1) * 2048, SMALL_WAVES * PLANES * 1024);      // codes of the rows and of the channels; the waves' sums take their place
+template <typename T>
+int launch_small8(const RingArgs& g, const T* x, int64_t ldx, int64_t K, hipStream_t st) {
+    SLIM_PROF("small8", st, (double)g.M * K * sizeof(T) + (double)g.N * g.units * 128 + (double)g.M * g.N * sizeof(T), 2.0 * g.M * g.N * K);
+    auto kernel = K <= 512 ? small8_kernel<T, 1> : K <= 1024 ? small8_kernel<T, 2> : small8_kernel<T, 4>;
+    const int bytes = max(g.units * 2 * 2048, SMALL_WAVES * 1024);      // codes of the rows and of the channels; the waves' sums take their place
     SLIM_HIP(slim_allow_dynamic_lds((const void*)kernel, bytes));
-    kernel<<<dim3((unsigned)ceil_div64(g.N, 16), (unsigned)ceil_div64(g.M, 16)), 64 * SMALL_WAVES, bytes, st>>>(g, x, ldx, (int)K, colscale);
+    kernel<<<dim3((unsigned)ceil_div64(g.N, 16), (unsigned)ceil_div64(g.M, 16)), 64 * SMALL_WAVES, bytes, st>>>(g, x, ldx, (int)K);
     SLIM_LAUNCH_CHECK();
     return SLIM_OK;
 }
@@ -1140,7 +928,7 @@ __global__ __launch_bounds__(512) void token8_kernel(const TokenArgs g) {
     for (int m = 0; m < M; ++m) {
         uint32_t top = 0;
         for (int i = 0; i < waves; ++i) top = max(top, part[i * M + m]);
-        const RowScale s = row_scale<1>(top);
+        const RowScale s = row_scale(top);
         scale[m] = s.scale;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
@@ -1150,7 +938,7 @@ __global__ __launch_bounds__(512) void token8_kernel(const TokenArgs g) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) keep[m][i][j] = 0.f;
             }
-            store_codes<1>(keep[m][i], s.inverse, (int8_t*)codes, ldl, m, c);
+            *(uint2*)(codes + m * ldl + c) = encode(keep[m][i], s.inverse);
         }
     }
     __syncthreads();
@@ -1240,11 +1028,6 @@ __global__ __launch_bounds__(256) void transpose8_kernel(const int8_t* __restric
 
 }  // namespace
 
-// the longest reduction whose sums of products of codes in [-128, 127] fit 32 bits
-#define SLIM_INT8_MAX_REDUCTION 131071
-// rows and columns: a workgroup of 256 threads each stays below a grid's 2^32 threads
-#define SLIM_INT8_MAX_DIM ((1 << 24) - 1)
-
 extern "C" int64_t slim_rows8_ld(int64_t K) { return K > 0 ? pad128(K) : 0; }
 
 extern "C" int slim_quantize_rows8(const void* x, int dtype, int64_t R, int64_t K, int64_t ldx, int8_t* codes, int64_t ldc, float* scale,
@@ -1255,7 +1038,7 @@ extern "C" int slim_quantize_rows8(const void* x, int dtype, int64_t R, int64_t 
     SLIM_REQUIRE(ldc >= pad128(K) && ldc % 16 == 0 && (uintptr_t)codes % 16 == 0,
                  "slim_quantize_rows8: rows of codes hold slim_rows8_ld(K) bytes and start at multiples of 16");
     SLIM_PROF("quantize_rows8", stream, (double)R * K * (element_size(dtype) + 1) + 4.0 * R);
-    return quantize_rows_any<1>(x, dtype, R, K, ldx, nullptr, codes, ldc, scale, (hipStream_t)stream);
+    return quantize_rows_any(x, dtype, R, K, ldx, codes, ldc, scale, (hipStream_t)stream);
 }
 
 extern "C" int slim_transpose8(const int8_t* codes, int64_t N, int64_t K, int64_t ld, int8_t* codes_t, int64_t ldt, void* stream) {
@@ -1268,7 +1051,7 @@ extern "C" int slim_transpose8(const int8_t* codes, int64_t N, int64_t K, int64_
 }
 
 extern "C" int64_t slim_gemm8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    return M > 0 && N > 0 && K > 0 && !takes_ring<1>(M, N) ? plan_gemm8<1>(M, N, pad128(K) / 128).slab_bytes() : 0;
+    return M > 0 && N > 0 && K > 0 && !takes_ring(M, N) ? plan_gemm8(M, N, pad128(K) / 128).slab_bytes() : 0;
 }
 
 extern "C" int slim_gemm8_nt(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, const float* sb, int64_t M, int64_t N,
@@ -1281,13 +1064,13 @@ extern "C" int slim_gemm8_nt(const int8_t* a, int64_t lda, const float* sa, cons
     SLIM_REQUIRE(workspace_bytes >= slim_gemm8_workspace_bytes(M, N, K) && (workspace || workspace_bytes == 0) && (uintptr_t)workspace % 16 == 0,
                  "slim_gemm8_nt: workspace too small or misaligned");
     SLIM_REQUIRE(lda < 1 << 23 && ldb < 1 << 23, "slim_gemm8_nt: rows of codes lie too far apart");
-    if (takes_ring<1>(M, N)) return launch_ring8<1>(RingArgs{a, lda, M, sa, b, ldb, sb, bias, out, ldo, dtype, M, N, (int)(pad128(K) / 128)}, (hipStream_t)stream);
-    Gemm8Args g{a, b, lda, ldb, M, M, N, (int)(pad128(K) / 128), sa, sb, bias, out, ldo, dtype, 0, 0, 1, 0, nullptr, 0};
-    return gemm8<1>(g, workspace, (hipStream_t)stream);
+    if (takes_ring(M, N)) return launch_ring8(RingArgs{a, lda, sa, b, ldb, sb, bias, out, ldo, dtype, M, N, (int)(pad128(K) / 128)}, (hipStream_t)stream);
+    Gemm8Args g{a, b, lda, ldb, M, N, (int)(pad128(K) / 128), sa, sb, bias, out, ldo, dtype, 0, 0, 1, 0, nullptr, 0};
+    return gemm8(g, workspace, (hipStream_t)stream);
 }
 
 extern "C" int64_t slim_linear8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    if (M <= 0 || N <= 0 || K <= 0 || token_waves(M, K) || takes_small<1>(M, N, K)) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || token_waves(M, K) || takes_small(M, N, K)) return 0;
     return align256(M * pad128(K)) + align256(M * 4) + slim_gemm8_workspace_bytes(M, N, K);
 }
 
@@ -1304,13 +1087,13 @@ extern "C" int slim_linear8_forward(const void* x, int dtype, int64_t ldx, int64
         if (dtype == SLIM_DTYPE_BF16) return token8<bf16_t>(g, M, waves, (hipStream_t)stream);
         return token8<_Float16>(g, M, waves, (hipStream_t)stream);
     }
-    if (takes_small<1>(M, N, K)) {
+    if (takes_small(M, N, K)) {
         SLIM_REQUIRE(known(dtype), "slim_linear8_forward: unknown element type %d", dtype);
         SLIM_REQUIRE(N <= SLIM_INT8_MAX_DIM && (uintptr_t)codes % 16 == 0, "slim_linear8_forward: weight too large or misaligned");
-        const RingArgs g{nullptr, 0, M, nullptr, codes, pad128(K), scale, bias, y, ldy, dtype, M, N, (int)(pad128(K) / 128)};
-        if (dtype == SLIM_DTYPE_F32) return launch_small8<float, 1>(g, (const float*)x, ldx, K, nullptr, (hipStream_t)stream);
-        if (dtype == SLIM_DTYPE_BF16) return launch_small8<bf16_t, 1>(g, (const bf16_t*)x, ldx, K, nullptr, (hipStream_t)stream);
-        return launch_small8<_Float16, 1>(g, (const _Float16*)x, ldx, K, nullptr, (hipStream_t)stream);
+        const RingArgs g{nullptr, 0, nullptr, codes, pad128(K), scale, bias, y, ldy, dtype, M, N, (int)(pad128(K) / 128)};
+        if (dtype == SLIM_DTYPE_F32) return launch_small8<float>(g, (const float*)x, ldx, K, (hipStream_t)stream);
+        if (dtype == SLIM_DTYPE_BF16) return launch_small8<bf16_t>(g, (const bf16_t*)x, ldx, K, (hipStream_t)stream);
+        return launch_small8<_Float16>(g, (const _Float16*)x, ldx, K, (hipStream_t)stream);
     }
     int8_t* xc = (int8_t*)workspace;
     float* sx = (float*)(xc + align256(M * pad128(K)));
@@ -1318,45 +1101,4 @@ extern "C" int slim_linear8_forward(const void* x, int dtype, int64_t ldx, int64
     if (rc) return rc;
     char* slab = (char*)sx + align256(M * 4);
     return slim_gemm8_nt(xc, pad128(K), sx, codes, pad128(K), scale, M, N, K, bias, dtype, y, ldy, slab, (char*)workspace + workspace_bytes - slab, stream);
-}
-
-extern "C" int64_t slim_linear8_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
-    if (M <= 0 || N <= 0 || K <= 0 || !known(dtype)) return 0;
-    if (planes_of(dtype) == 3 ? takes_small<3>(M, K, N) : takes_small<2>(M, K, N)) return 0;
-    const int64_t rows = (M + 15) / 16 * 16 * planes_of(dtype);
-    const bool ring = planes_of(dtype) == 3 ? takes_ring<3>(M, K) : takes_ring<2>(M, K);
-    return align256(rows * pad128(N)) + align256(M * 4) +
-           (ring ? 0 : (planes_of(dtype) == 3 ? plan_gemm8<3>(rows, K, pad128(N) / 128) : plan_gemm8<2>(rows, K, pad128(N) / 128)).slab_bytes());
-}
-
-extern "C" int slim_linear8_backward(const void* dy, int dtype, int64_t lddy, int64_t M, int64_t N, const int8_t* codes_t, const float* scale, int64_t K,
-                                     void* dx, int64_t lddx, void* workspace, int64_t workspace_bytes, void* stream) {
-    SLIM_REQUIRE(dy && codes_t && scale && dx && M > 0 && N > 0 && K > 0 && lddy >= N && lddx >= K, "slim_linear8_backward: bad arguments");
-    SLIM_REQUIRE(known(dtype), "slim_linear8_backward: unknown element type %d", dtype);
-    SLIM_REQUIRE(N <= SLIM_INT8_MAX_REDUCTION && M <= SLIM_INT8_MAX_DIM && K <= SLIM_INT8_MAX_DIM, "slim_linear8_backward: too large");
-    const int64_t need = slim_linear8_backward_workspace_bytes(M, N, K, dtype);
-    SLIM_REQUIRE(workspace_bytes >= need && (workspace || !need) && (uintptr_t)workspace % 16 == 0,
-                 "slim_linear8_backward: workspace too small or misaligned");
-    SLIM_REQUIRE((uintptr_t)codes_t % 16 == 0, "slim_linear8_backward: codes must be 16-byte aligned");
-    hipStream_t st = (hipStream_t)stream;
-    const int planes = planes_of(dtype);
-    const int64_t rows = (M + 15) / 16 * 16 * planes, ld = pad128(N);
-    if (!need) {
-        const RingArgs g{nullptr, 0, M, nullptr, codes_t, ld, nullptr, nullptr, dx, lddx, dtype, M, K, (int)(ld / 128)};
-        if (dtype == SLIM_DTYPE_F32) return launch_small8<float, 3>(g, (const float*)dy, lddy, N, scale, st);
-        if (dtype == SLIM_DTYPE_BF16) return launch_small8<bf16_t, 2>(g, (const bf16_t*)dy, lddy, N, scale, st);
-        return launch_small8<_Float16, 2>(g, (const _Float16*)dy, lddy, N, scale, st);
-    }
-    int8_t* q = (int8_t*)workspace;
-    float* sq = (float*)(q + align256(rows * ld));
-    const int rc = planes == 3 ? quantize_rows_any<3>(dy, dtype, M, N, lddy, scale, q, ld, sq, st)
-                               : quantize_rows_any<2>(dy, dtype, M, N, lddy, scale, q, ld, sq, st);
-    if (rc) return rc;
-    if (planes == 3 ? takes_ring<3>(M, K) : takes_ring<2>(M, K)) {
-        const RingArgs g{q, ld, rows, sq, codes_t, ld, nullptr, nullptr, dx, lddx, dtype, M, K, (int)(ld / 128)};
-        return planes == 3 ? launch_ring8<3>(g, st) : launch_ring8<2>(g, st);
-    }
-    void* slab = (char*)sq + align256(M * 4);
-    Gemm8Args g{q, codes_t, ld, ld, rows, M, K, (int)(ld / 128), sq, nullptr, nullptr, dx, lddx, dtype, 0, 0, 1, 0, nullptr, 0};
-    return planes == 3 ? gemm8<3>(g, slab, st) : gemm8<2>(g, slab, st);
 }

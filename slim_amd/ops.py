@@ -1240,8 +1240,9 @@ def linear8_forward(x, codes, scale, bias=None):
 
 def linear8_backward(dy, codes_t, scale):
     """dx [M, K] = (dy [M, N] * scale) @ codes: the gradient of linear8_forward with respect to x, the quantisation of x passed
-    straight through.  codes_t [K, Np] from transpose8; dx has the type of dy.  dy * scale is kept as integers of 16 bits per row
-    (24 for fp32), so a row's error is below sqrt(N / 12) 2^-15 (2^-23) of its norm."""
+    straight through.  codes_t [K, Np] from transpose8; dx has the type of dy.  dy * scale is a float for every element, kept to 2^-23
+    of itself (fp32: all 24 bits) over a range of 2^50 (2^61) below the row's largest; sums are fp32.  A row's gradient does not
+    depend on the rows beside it."""
     dy, M, N, ld, dt, gpu = _rows8(dy, "dy")
     codes_t, K, Np = _codes8(codes_t, gpu, "codes_t")
     if Np != _pad128(N):
