@@ -175,6 +175,7 @@ class Int8Linear(torch.nn.Module):
     its codes exactly; any other weight is quantised here, one scale per output channel (ops.quantize_rows8).  The activation
     is quantised token by token on every call.  Adapters (lora_left, lora_right, lora_rank, lora_quantizer, lora_left_mask) and
     forward hooks of the linear carry over; its input fake-quantisation pre-hooks do not (the input is quantised here).
+    Derivatives are backward-mode: a forward-mode dual tensor is refused.
     As with PackedLinear the tensors are plain attributes: `model.to(dtype)` does not change them."""
 
     TENSORS = ("codes", "scale", "bias", "lora_left", "lora_right", "lora_left_mask")
@@ -273,6 +274,8 @@ class Int8Linear(torch.nn.Module):
         if torch.is_autocast_enabled("cuda") and x.dtype in (torch.float32, torch.bfloat16, torch.float16):
             x = x.to(torch.get_autocast_dtype("cuda"))
         x2 = x.reshape(-1, self.in_features)
+        if torch.autograd.forward_ad.unpack_dual(x2).tangent is not None:
+            raise NotImplementedError("Int8Linear has no forward-mode derivative (backward mode only)")
         y = _Int8Product.apply(x2, self) if torch.is_grad_enabled() and x2.requires_grad else self.product(x2)
         return y.reshape(*x.shape[:-1], self.out_features)
 
