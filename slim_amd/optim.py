@@ -115,17 +115,30 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """torch's, with the state's own element types (which it would change to the parameters').  What torch.optim.AdamW saved over
-        fp32 parameters loads too (its moments continue in 32 bits)."""
-        super().load_state_dict(state_dict)
-        for group in self.param_groups:
-            for name in ("state_bits", "master_weights"):
-                group.setdefault(name, self.defaults[name])
-        for state in self.state.values():
-            state["step"] = int(state["step"])
-        ids = [i for group in state_dict["param_groups"] for i in group["params"]]
-        params = [p for group in self.param_groups for p in group["params"]]
-        for i, p in zip(ids, params):
-            for name in _STATE_TENSORS:
-                saved = state_dict["state"].get(i, {}).get(name)
-                if saved is not None:
-                    self.state[p][name] = saved.detach().to(p.device, copy=True).contiguous()
+        fp32 parameters loads too (its moments continue in 32 bits).  Registered pre-hooks decide what is loaded, post-hooks see the
+        state as it stays."""
+        seen = {}
+
+        def take(_, final):                              # behind every other pre-hook: the dictionary that is loaded
+            seen.update(final)
+
+        def repair(_):                                   # in front of every other post-hook
+            for group in self.param_groups:
+                for name in ("state_bits", "master_weights"):
+                    group.setdefault(name, self.defaults[name])
+            ids = [i for group in seen["param_groups"] for i in group["params"]]
+            params = [p for group in self.param_groups for p in group["params"]]
+            for i, p in zip(ids, params):
+                saved = seen["state"].get(i)
+                if saved is None:
+                    continue
+                self.state[p]["step"] = int(saved["step"])
+                for name in _STATE_TENSORS:
+                    if saved.get(name) is not None:
+                        self.state[p][name] = saved[name].detach().to(p.device, copy=True).contiguous()
+        handles = self.register_load_state_dict_pre_hook(take), self.register_load_state_dict_post_hook(repair, prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for handle in handles:
+                handle.remove()

@@ -1,0 +1,47 @@
+"""The optimizer's bookkeeping, on the CPU: nothing is launched."""
+import copy
+
+import pytest
+import torch
+
+from slim_amd.optim import AdamW
+
+
+def parameter(n=8, dtype=torch.bfloat16):
+    return torch.nn.Parameter(torch.zeros(n, dtype=dtype))
+
+
+def with_state(opt, value=1.0):
+    """`opt` as after five steps, its moments at `value`."""
+    for group in opt.param_groups:
+        for p in group["params"]:
+            opt.state[p] = dict(step=5, exp_avg=torch.full(p.shape, value), exp_avg_sq=torch.full(p.shape, value))
+    return opt
+
+
+def test_load_hooks_decide_what_is_loaded():
+    saved = with_state(AdamW([parameter()])).state_dict()
+    p = parameter()
+    opt, seen = AdamW([p]), []
+
+    def pre(_, state_dict):
+        state_dict = copy.deepcopy(state_dict)
+        state_dict["state"][0]["exp_avg"] += 6
+        state_dict["state"][0]["step"] = torch.tensor(9.0)
+        return state_dict
+
+    def post(o):
+        seen.append({k: v if k == "step" else v.dtype for k, v in o.state[p].items()})
+    hooks = opt.register_load_state_dict_pre_hook(pre), opt.register_load_state_dict_post_hook(post)
+    opt.load_state_dict(saved)
+    assert bool((opt.state[p]["exp_avg"] == 7).all()) and bool((opt.state[p]["exp_avg_sq"] == 1).all()) and opt.state[p]["step"] == 9
+    assert seen == [dict(step=9, exp_avg=torch.float32, exp_avg_sq=torch.float32)]       # (not the parameter's bf16)
+    assert bool((saved["state"][0]["exp_avg"] == 1).all())
+    for hook in hooks:
+        hook.remove()
+    opt.load_state_dict(saved)
+    assert bool((opt.state[p]["exp_avg"] == 1).all()) and len(seen) == 1
+    with pytest.raises(ValueError, match="parameter group"):
+        opt.load_state_dict(AdamW([parameter(), parameter()]).state_dict())
+    assert bool((opt.state[p]["exp_avg"] == 1).all()) and opt.state[p]["step"] == 5
+    assert not opt._optimizer_load_state_dict_pre_hooks and not opt._optimizer_load_state_dict_post_hooks       # (none of its own stays)
