@@ -8,6 +8,8 @@ from . import ops
 # tensors with fewer elements keep 32-bit moments when state_bits is 8 (norm weights and biases: nothing to save there)
 MIN_8BIT_NUMEL = 4096
 _STATE_TENSORS = ("exp_avg", "exp_avg_sq", "scales", "master")
+# what torch's Adam and AdamW record where their update is not this one (an Adam without weight decay is)
+_OTHER_UPDATES = {"amsgrad": True, "maximize": True, "decoupled_weight_decay": False}
 
 
 class AdamW(torch.optim.Optimizer):
@@ -115,11 +117,15 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """torch's, with the state's own element types (which it would change to the parameters').  What torch.optim.AdamW saved over
-        fp32 parameters loads too (its moments continue in 32 bits).  Registered pre-hooks decide what is loaded, post-hooks see the
+        fp32 parameters loads too (its moments continue in 32 bits), but for amsgrad and maximize.  Registered pre-hooks decide what is loaded, post-hooks see the
         state as it stays."""
         seen = {}
 
         def take(_, final):                              # behind every other pre-hook: the dictionary that is loaded
+            for group in final["param_groups"]:
+                for name, value in _OTHER_UPDATES.items():
+                    if group.get(name) == value and (name != "decoupled_weight_decay" or group.get("weight_decay")):
+                        raise ValueError(f"AdamW cannot continue a state of another update: {name}={value}")
             seen.update(final)
 
         def repair(_):                                   # in front of every other post-hook

@@ -45,3 +45,22 @@ def test_load_hooks_decide_what_is_loaded():
         opt.load_state_dict(AdamW([parameter(), parameter()]).state_dict())
     assert bool((opt.state[p]["exp_avg"] == 1).all()) and opt.state[p]["step"] == 5
     assert not opt._optimizer_load_state_dict_pre_hooks and not opt._optimizer_load_state_dict_post_hooks       # (none of its own stays)
+
+
+@pytest.mark.parametrize("cls,kw,refused", [("AdamW", {}, False), ("AdamW", dict(amsgrad=True), True), ("AdamW", dict(maximize=True), True),
+                                            ("Adam", dict(weight_decay=0.1), True), ("Adam", {}, False), ("AdamW", dict(fused=True), False)])
+def test_states_of_another_update_are_refused(cls, kw, refused):
+    """Not continued as if they were plain AdamW's: the sign of the step, or the second moment it divides by, would change."""
+    q = parameter(dtype=torch.float32)
+    other = getattr(torch.optim, cls)([q], lr=1e-2, **kw)
+    q.grad = torch.ones_like(q)
+    other.step()
+    p = parameter(dtype=torch.float32)
+    opt = with_state(AdamW([p]), 3.0)
+    if refused:
+        with pytest.raises(ValueError, match="another update"):
+            opt.load_state_dict(other.state_dict())
+        assert opt.state[p]["step"] == 5 and bool((opt.state[p]["exp_avg"] == 3).all())
+    else:
+        opt.load_state_dict(other.state_dict())
+        assert opt.state[p]["step"] == 1 and torch.equal(opt.state[p]["exp_avg"], other.state[q]["exp_avg"])
