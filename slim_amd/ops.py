@@ -1258,6 +1258,7 @@ def linear8_backward(dy, codes_t, scale):
 
 # ---- AdamW over many tensors ----------------------------------------------------------------------------------
 ADAMW_BLOCK = 512         # elements of a tensor that share a pair of scales (8-bit moments)
+ADAMW_MAX_NUMEL = 2048 << 23      # elements of a tensor, at most
 
 
 def _alike(tensors, dtype, index, sizes, name):
@@ -1342,13 +1343,27 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, beta1=0.9, bet
     position in it.  masters: fp32 copies of 16-bit parameters, which are then their roundings.  No two tensors that are updated overlap.  norm (0-d fp32 tensor, grad_norm) with max_norm: the gradients are
     multiplied by min(1, max_norm / (norm + 1e-6)) as they are read.  step counts from 1; eps is 0 or at least 2^-126.  Empty tensors are left alone.  A captured call
     replays with the step, lr and seed that it was captured with."""
+    _adamw_run(_adamw_plan(params, grads, exp_avgs, exp_avg_sqs, step=step, lr=lr, beta1=beta1, beta2=beta2, eps=eps, weight_decay=weight_decay, scales=scales,
+                         masters=masters, seed=seed, norm=norm, max_norm=max_norm, first_index=first_index))
+
+
+def _adamw_plan(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0, scales=None, masters=None,
+               seed=0, norm=None, max_norm=None, first_index=0):
+    """The checks of adamw_step: what _adamw_run takes (None: nothing to update).  Nothing that passes them is refused by _adamw_run, so an
+    optimizer whose step takes several calls can plan them all before it updates anything."""
+    if not (step >= 1 and lr >= 0 and 0 <= beta1 < 1 and 0 <= beta2 < 1 and weight_decay >= 0 and first_index >= 0):
+        raise ValueError("adamw_step: step counts from 1, betas lie in [0, 1), lr, eps and weight_decay are not negative")
+    if eps != 0 and not eps >= 2.0 ** -126:
+        raise ValueError(f"adamw_step: eps is 0 or at least 2^-126, got {eps}")
+    if max_norm is not None and not max_norm > 0:
+        raise ValueError(f"adamw_step: max_norm must be positive, got {max_norm}")
     params, grads, ms, vs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
     ss, ws = None if scales is None else list(scales), None if masters is None else list(masters)
     count = len(params)
     if not count == len(grads) == len(ms) == len(vs) or ss is not None and len(ss) != count or ws is not None and len(ws) != count:
         raise ValueError("adamw_step: all lists must be equally long")
     if not count:
-        return
+        return None
     gpu = _gpu_of(params[0], "params")
     dtype = params[0].dtype
     dt = _DTYPES.get(dtype)
@@ -1381,13 +1396,24 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, *, step, lr, beta1=0.9, bet
         params, grads, ms, vs, ss, ws = (None if x is None else [x[i] for i in keep] for x in (params, grads, ms, vs, ss, ws))
         sizes = [sizes[i] for i in keep]
         if not keep:
-            return
+            return None
+    if max(sizes) > ADAMW_MAX_NUMEL:
+        raise ValueError(f"adamw_step: a tensor holds {max(sizes)} elements, at most {ADAMW_MAX_NUMEL} are supported")
     addresses = [*map(torch.Tensor.data_ptr, itertools.chain(grads, params, ms, vs, ss or (), ws or ()))]
     if len(set(addresses[len(grads):])) < len(addresses) - len(grads):
         raise ValueError("adamw_step: a tensor that is updated is in the lists twice")
     words, at = _words(addresses + sizes)                                # one array after another
     size, end = 8 * len(params), at + 8 * len(addresses)
-    _call_at(gpu, "slim_adamw_step", at + size, at, at + 2 * size, at + 3 * size, None if ss is None else at + 4 * size, None if ws is None else end - size, end,
-             len(params), dt, int(first_index), int(step), float(lr), float(beta1), float(beta2), float(eps),
-             float(weight_decay), _p(norm), 0.0 if max_norm is None else float(max_norm), int(seed) & 0xffffffff)
+    args = (at + size, at, at + 2 * size, at + 3 * size, None if ss is None else at + 4 * size, None if ws is None else end - size, end, len(params), dt,
+            int(first_index), int(step), float(lr), float(beta1), float(beta2), float(eps), float(weight_decay), _p(norm),
+            0.0 if max_norm is None else float(max_norm), int(seed) & 0xffffffff)
+    return gpu, args, params, (words, grads, ms, vs, ss, ws, norm)       # (what the addresses point to lives as long as the plan)
+
+
+def _adamw_run(plan):
+    """The update that _adamw_plan checked, on the current stream; a plan is run once, at once."""
+    if plan is None:
+        return
+    gpu, args, params, _ = plan
+    _call_at(gpu, "slim_adamw_step", *args)
     torch.autograd.graph.increment_version(params)

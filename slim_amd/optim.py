@@ -91,25 +91,27 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("AdamW updates parameters of one GPU")
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW.step counts steps on the host and cannot be captured; ops.grad_norm and ops.adamw_step can")
-        norm = self.last_norm = None if self.max_grad_norm is None else self._norm(items)
+        norm = None if self.max_grad_norm is None else self._norm(items)
         calls = {}
         for p, group, g in items:
-            state = self.state[p]
-            if not state:
-                state.update(self._new_state(p, group))
+            state = self.state.get(p) or self._new_state(p, group)       # (a new one is kept once nothing can be refused any more)
             key = (id(group), p.dtype, "scales" in state, "master" in state, state["step"] + 1)
             calls.setdefault(key, (group, []))[1].append((p, g, state))
-        first = 0
+        plans, first = [], 0
         for (_, _, eight, master, step), (group, members) in calls.items():
             states = [s for _, _, s in members]
-            ops.adamw_step([p for p, _, _ in members], [g for _, g, _ in members], [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
-                           step=step, lr=float(group["lr"]), beta1=group["betas"][0], beta2=group["betas"][1], eps=group["eps"],
-                           weight_decay=group["weight_decay"], scales=[s["scales"] for s in states] if eight else None,
-                           masters=[s["master"] for s in states] if master else None, seed=self.seed + step * 0x9e3779b1, norm=norm,
-                           max_norm=self.max_grad_norm, first_index=first)
+            plans.append(ops._adamw_plan([p for p, _, _ in members], [g for _, g, _ in members], [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
+                                        step=step, lr=float(group["lr"]), beta1=group["betas"][0], beta2=group["betas"][1], eps=group["eps"],
+                                        weight_decay=group["weight_decay"], scales=[s["scales"] for s in states] if eight else None,
+                                        masters=[s["master"] for s in states] if master else None, seed=self.seed + step * 0x9e3779b1, norm=norm,
+                                        max_norm=self.max_grad_norm, first_index=first))
             first += len(members)
-            for state in states:
+        self.last_norm = norm
+        for plan, ((*_, step), (_, members)) in zip(plans, calls.items()):
+            ops._adamw_run(plan)
+            for p, _, state in members:
                 state["step"] = step
+                self.state[p] = state
         return loss
 
     def __getstate__(self):
