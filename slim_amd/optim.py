@@ -17,11 +17,13 @@ class AdamW(torch.optim.Optimizer):
 
     state_bits: 32, or 8: first moments as e4m3 and second as e5m2 numbers with a pair of scales per 512 elements, rounded
     stochastically (an exponential average that moves by 0.1 % a step would stand still under rounding to nearest); the random
-    bits are a function of `seed`, the step and the position, so a run can be repeated exactly.  Tensors below
-    MIN_8BIT_NUMEL elements keep 32-bit moments.
+    bits are a function of `seed`, the step and the position, so a run can be repeated exactly; `seed` is an option of the groups
+    and so part of state_dict(): a run that is loaded goes on with its own.  Tensors below MIN_8BIT_NUMEL elements keep
+    32-bit moments.
     master_weights: 16-bit parameters keep an fp32 copy that is what is updated.
     max_grad_norm: gradients are multiplied by min(1, max_grad_norm / (norm + 1e-6)) as they are read, norm over all parameters
-    of all groups; the gradients themselves stay as they were.  `last_norm` is that norm after a step (a 0-d tensor on the GPU).
+    of all groups; the gradients themselves stay as they were.  `last_norm` is that norm after a step (a 0-d tensor on the GPU).  It is not part
+    of state_dict(): a run that is loaded needs it passed again.
 
     step() cannot be captured into a graph: it counts on the host.  (ops.grad_norm and ops.adamw_step can.)"""
 
@@ -38,9 +40,12 @@ class AdamW(torch.optim.Optimizer):
         if max_grad_norm is not None and not max_grad_norm > 0:
             raise ValueError(f"max_grad_norm must be positive, got {max_grad_norm}")
         self.max_grad_norm = max_grad_norm
-        self.seed = int(seed)
         self.last_norm = None
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, master_weights=master_weights))
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, master_weights=master_weights, seed=int(seed)))
+
+    @property
+    def seed(self):
+        return self.param_groups[0]["seed"]
 
     def _new_state(self, p, group):
         state = dict(step=0)
@@ -103,7 +108,7 @@ class AdamW(torch.optim.Optimizer):
             plans.append(ops._adamw_plan([p for p, _, _ in members], [g for _, g, _ in members], [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
                                         step=step, lr=float(group["lr"]), beta1=group["betas"][0], beta2=group["betas"][1], eps=group["eps"],
                                         weight_decay=group["weight_decay"], scales=[s["scales"] for s in states] if eight else None,
-                                        masters=[s["master"] for s in states] if master else None, seed=self.seed + step * 0x9e3779b1, norm=norm,
+                                        masters=[s["master"] for s in states] if master else None, seed=group["seed"] + step * 0x9e3779b1, norm=norm,
                                         max_norm=self.max_grad_norm, first_index=first))
             first += len(members)
         self.last_norm = norm
@@ -115,7 +120,7 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def __getstate__(self):
-        return dict(super().__getstate__(), max_grad_norm=self.max_grad_norm, seed=self.seed, last_norm=self.last_norm)
+        return dict(super().__getstate__(), max_grad_norm=self.max_grad_norm, last_norm=self.last_norm)
 
     def load_state_dict(self, state_dict):
         """torch's, with the state's own element types (which it would change to the parameters').  What torch.optim.AdamW saved over
@@ -132,7 +137,7 @@ class AdamW(torch.optim.Optimizer):
 
         def repair(_):                                   # in front of every other post-hook
             for group in self.param_groups:
-                for name in ("state_bits", "master_weights"):
+                for name in ("state_bits", "master_weights", "seed"):
                     group.setdefault(name, self.defaults[name])
             ids = [i for group in seen["param_groups"] for i in group["params"]]
             params = [p for group in self.param_groups for p in group["params"]]

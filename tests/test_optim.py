@@ -64,3 +64,14 @@ def test_states_of_another_update_are_refused(cls, kw, refused):
     else:
         opt.load_state_dict(other.state_dict())
         assert opt.state[p]["step"] == 1 and torch.equal(opt.state[p]["exp_avg"], other.state[q]["exp_avg"])
+
+
+def test_the_seed_is_saved():
+    saved = with_state(AdamW([parameter()], seed=7)).state_dict()
+    opt = AdamW([parameter()], seed=8)
+    opt.load_state_dict(saved)
+    assert [g["seed"] for g in opt.param_groups] == [7] and opt.seed == 7
+    q = parameter(dtype=torch.float32)
+    opt = AdamW([parameter(dtype=torch.float32)], seed=8)
+    opt.load_state_dict(torch.optim.AdamW([q]).state_dict())               # (which has none)
+    assert [g["seed"] for g in opt.param_groups] == [8]

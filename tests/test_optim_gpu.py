@@ -58,3 +58,21 @@ def test_a_refused_step_changes_nothing(AdamW, damage):
             opt.step()
         runs.append(contents(opt, ps))
     assert same(*runs)
+
+
+def test_a_loaded_run_goes_on_with_its_own_random_bits(AdamW):
+    """Saved by an optimizer of seed 4, loaded into one made without: the same codes, bit for bit."""
+    runs = []
+    for resumed in (False, True):
+        g = torch.Generator().manual_seed(5)
+        p = torch.nn.Parameter(torch.randn(6000, generator=g).to(DEV))
+        opt = AdamW([p], state_bits=8, seed=4)
+        for step in range(4):
+            if step == 2 and resumed:
+                saved = opt.state_dict()
+                opt = AdamW([p], state_bits=8)
+                opt.load_state_dict(saved)
+            p.grad = torch.randn(6000, generator=g).to(DEV)
+            opt.step()
+        runs.append(contents(opt, [p]))
+    assert same(*runs)
