@@ -580,12 +580,14 @@ int64_t slim_adamw_blocks(int64_t numel);
 /* g' = g * min(1, max_norm / (norm[0] + 1e-6)) (norm NULL: g); m = beta1 m + (1 - beta1) g'; v = beta2 v + (1 - beta2) g'^2;
  * w = w (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v / (1 - beta2^step)) + eps), in fp32.
  * scales NULL: exp_avg and exp_avg_sq are fp32.  Otherwise they are codes, e4m3 and e5m2 (the finite formats of the Open Compute
- * Project), times scales[block][0] and scales[block][1] (fp32, updated): block maximum / 448 and / 57344.  New codes are rounded
+ * Project), times scales[block][0] and scales[block][1] (fp32, updated): block maximum / 448 and / 57344, at least 2^-126 unless
+ * the block is zero.  New codes are rounded
  * up with probability equal to the value's place between its neighbours, with random bits that are a function of seed, the
  * tensor's ordinal first_index + i, and the position; a positive second moment never gets the code 0; a block that holds an
  * infinity or a NaN gets the scale NaN.
  * masters (16-bit parameters only) NULL: w is the parameter.  Otherwise w is masters[i] (fp32), and the parameter its rounding.
- * eps: 0 (an element whose gradients have all been 0 then becomes NaN, as 0 / 0 is) or at least 2^-126.  Tensors do not overlap. */
+ * eps: 0 (an element whose second moment is 0 then becomes NaN, as 0 / 0 is, or infinite where gradients below 2^-70 left it 0) or
+ * at least 2^-126.  Tensors do not overlap. */
 int slim_adamw_step(void* const* params, const void* const* grads, void* const* exp_avg, void* const* exp_avg_sq, float* const* scales,
                     float* const* masters, const int64_t* numel, int count, int dtype, int first_index, int64_t step, double lr, double beta1,
                     double beta2, double eps, double weight_decay, const float* norm, double max_norm, uint32_t seed, void* stream);

@@ -233,10 +233,13 @@ struct Scale {
     float scale, inverse;
     bool none;
 };
+// maximum / top, but 2^-126 at least, so that the scale and its reciprocal are normal numbers: then the codes are fixed point, down to
+// 2^-142 in the second moment, and what is positive below that takes its smallest code.  (A second moment lost beside a first one that is
+// kept would be a division by eps alone.)
 __device__ __forceinline__ Scale scale_for(uint32_t max_bits, float top) {
-    const float a = __uint_as_float(max_bits);
-    const bool bad = max_bits >= 0x7f800000u, none = bad || a < 0x1p-100f;
-    return {bad ? __uint_as_float(0x7fc00000u) : none ? 0.f : a / top, none ? 0.f : top / a, none};
+    const float a = __uint_as_float(max_bits), s = a / top;
+    const bool bad = max_bits >= 0x7f800000u, none = bad || max_bits == 0, low = s < 0x1p-126f;
+    return {bad ? __uint_as_float(0x7fc00000u) : none ? 0.f : low ? 0x1p-126f : s, none ? 0.f : low ? 0x1p126f : top / a, none};
 }
 
 // Per element: g *= clip; m = b1 m + c1 g; v = b2 v + c2 g^2; w = w (1 - lr decay) - rate m / (sqrt(v) root + eps).  A wave takes 512
