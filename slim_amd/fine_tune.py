@@ -43,6 +43,9 @@ def _mask_weight(module, inputs):
     module.weight.data[module.weight_mask] = 0
 
 
+_mask_weight.needless_in_int8 = True          # (packed.Int8Linear holds no weight, and its codes are frozen)
+
+
 # The reference re-stores the frozen weights and biases of the adapter layers as fp16 (fine_tune.py:31-33).  For the compressed
 # values (bf16 numbers of ordinary magnitude) that changes the container, not the values -- but a bf16 model then only runs
 # under autocast: outside it F.linear refuses bf16 activations with an fp16 weight, so the reference's own evaluation after
@@ -57,7 +60,7 @@ def disable_linear_layer_grads(model):
     The mask lives on the weight's device (the reference keeps it on the CPU and indexes the device tensor with it).
     Int8Linear modules (slim_amd.packed) hold no trainable weight; their pruned adapters are re-zeroed the same way."""
     for _, module in model.named_modules():
-        if type(module).__name__ == "Int8Linear" and hasattr(module, "lora_left_mask"):
+        if type(module).__name__ == "Int8Linear" and hasattr(module, "lora_left_mask") and _mask_lora not in module._forward_pre_hooks.values():
             module.register_forward_pre_hook(_mask_lora)
         if type(module).__name__ not in KNOWN_MODULES:
             continue

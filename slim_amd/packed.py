@@ -174,7 +174,8 @@ class Int8Linear(torch.nn.Module):
     A weight that lies on a per-tensor grid of at most 8 bits (what prune_and_quantize leaves: values code / scaling_factor) keeps
     its codes exactly; any other weight is quantised here, one scale per output channel (ops.quantize_rows8).  The activation
     is quantised token by token on every call.  Adapters (lora_left, lora_right, lora_rank, lora_quantizer, lora_left_mask) and
-    forward hooks of the linear carry over; its input fake-quantisation pre-hooks do not (the input is quantised here).
+    hooks of the linear carry over, but for input fake-quantisation (the input is quantised here) and the mask of a trained
+    weight (fine_tune; the codes are frozen).
     Derivatives are backward-mode: a forward-mode dual tensor is refused.
     As with PackedLinear the tensors are plain attributes: `model.to(dtype)` does not change them."""
 
@@ -194,8 +195,19 @@ class Int8Linear(torch.nn.Module):
         for name in ("lora_left", "lora_right", "lora_rank", "lora_quantizer", "lora_left_mask"):
             if hasattr(lin, name):
                 setattr(self, name, getattr(lin, name))
-        for hook_id, hook in lin._forward_hooks.items():
-            self._forward_hooks[hook_id] = hook
+        self._take_hooks(lin)
+
+    def _take_hooks(self, lin):
+        """The linear's hooks with their marks, but for those that the module itself makes needless (input fake-quantisation, the mask
+        of a trained weight)."""
+        for name in ("_forward_hooks", "_forward_hooks_with_kwargs", "_forward_hooks_always_called", "_forward_pre_hooks", "_forward_pre_hooks_with_kwargs",
+                     "_backward_hooks", "_backward_pre_hooks"):
+            getattr(self, name).update(getattr(lin, name))
+        self._is_full_backward_hook = lin._is_full_backward_hook
+        for hook_id, hook in list(self._forward_pre_hooks.items()):
+            if getattr(hook, "needless_in_int8", False):
+                del self._forward_pre_hooks[hook_id]
+                self._forward_pre_hooks_with_kwargs.pop(hook_id, None)
 
     @staticmethod
     def _codes_of(W, sf):

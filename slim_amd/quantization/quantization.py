@@ -144,6 +144,7 @@ def attach_input_quantization_hooks(model, num_bits=8, input_group_size=-1, bitw
             else:
                 deq = ops.input_fake_quant_fp8(x)
             input[0].data = deq
+    input_quantization_pre_hook.needless_in_int8 = True          # (packed.Int8Linear quantises its input itself)
 
     for layer in get_layers_list(model):
         for lin in find_layers(layer).values():

@@ -35,3 +35,41 @@ def test_forward_mode_derivatives_are_refused(layer):
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(layer, (x,), (t,))
     assert torch.allclose(layer(x), x @ layer.dense_weight().t(), atol=1e-5)
+
+
+def test_hooks_of_the_linear_carry_over(layer):
+    """Forward hooks and pre-hooks of either signature, those of the adapters' mask among them; not those whose work is done here."""
+    from slim_amd.fine_tune import disable_linear_layer_grads
+    from slim_amd.quantization.quantization import attach_input_quantization_hooks
+    model = torch.nn.Module()
+    model.model = torch.nn.Module()
+    model.model.layers = torch.nn.ModuleList([torch.nn.Sequential(torch.nn.Linear(K, N), torch.nn.Linear(K, N))])
+    adapted, plain = model.model.layers[0]
+    adapted.lora_left = torch.nn.Parameter(torch.ones(K, 2))
+    adapted.lora_right = torch.nn.Parameter(torch.ones(2, N))
+    adapted.lora_left_mask = torch.zeros(K, 2, dtype=torch.bool)
+    adapted.lora_left_mask[3] = True
+    attach_input_quantization_hooks(model)
+    disable_linear_layer_grads(model)
+    seen = []
+    adapted.register_forward_pre_hook(lambda module, args: seen.append("pre"))
+    adapted.register_forward_pre_hook(lambda module, args, kwargs: seen.append(("pre", dict(kwargs))), with_kwargs=True)
+    adapted.register_forward_hook(lambda module, args, out: seen.append("post"))
+    adapted.register_forward_hook(lambda module, args, kwargs, out: out + 1, with_kwargs=True)
+    adapted.register_full_backward_hook(lambda module, grad_in, grad_out: seen.append("backward"))
+    adapted.register_forward_hook(lambda module, args, out: seen.append("always"), always_call=True)
+    x = torch.randn(3, K)
+    before = layer(x)
+    layer.lora_left, layer.lora_left_mask = adapted.lora_left, adapted.lora_left_mask
+    layer._take_hooks(adapted)
+    with torch.no_grad():
+        y = layer(x)
+    assert seen == ["pre", ("pre", {}), "post", "always"] and torch.equal(y, before + 1)
+    assert bool((layer.lora_left[3] == 0).all()) and bool((layer.lora_left[:3] == 1).all())
+    with pytest.raises(ValueError, match="channels"):
+        layer(x[:, 1:])
+    assert seen[4:] == ["pre", ("pre", {}), "always"]
+    assert len(layer._backward_hooks) == 1 and layer._is_full_backward_hook
+    other = Int8Linear.from_tensors(dict(codes=layer.codes, scale=layer.scale), N, K, "cpu")
+    other._take_hooks(plain)                                 # an input quantiser and the mask of a trained weight: neither is called
+    assert torch.equal(other(x), before) and len(plain._forward_pre_hooks) == 2 and not other._forward_pre_hooks
