@@ -265,14 +265,21 @@ class Int8Linear(torch.nn.Module):
         return self.codes[:, :self.in_features].float() * self.scale[:, None]
 
     def transposed(self):
-        """The codes in the order of the backward pass, laid out on its first use and kept (as large as the codes)."""
-        if self._codes_t is None:
+        """The codes in the order of the backward pass, laid out on its first use and kept until drop_transposed(), or until the codes are
+        replaced or changed in place: a second byte per weight element, which packed_bytes does not count."""
+        version = None if self.codes.is_inference() else self.codes._version
+        if self._codes_t is None or self._codes_t[0] is not self.codes or self._codes_t[1] != version:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("Int8Linear: the first backward pass lays out the transposed codes and cannot be captured; run one eagerly, "
                                    "or call transposed() before the capture")
-            self._codes_t = ops.transpose8(self.codes, self.in_features)
+            self._codes_t = self.codes, version, ops.transpose8(self.codes, self.in_features)
             torch.cuda.current_stream(self.codes.device).synchronize()       # (whatever stream uses them next)
-        return self._codes_t
+        return self._codes_t[2]
+
+    def drop_transposed(self):
+        """Give the memory of transposed() back, after training; a later backward pass lays it out again.  (Not while a captured
+        backward pass is still to be replayed: it reads that memory.)"""
+        self._codes_t = None
 
     def product(self, x2):
         bias = self.bias

@@ -40,3 +40,34 @@ def test_pruned_adapters_stay_pruned_when_packed_late():
     with torch.no_grad():
         m(torch.randn(5, 64, device=DEV).bfloat16())
     assert not bool(m.lora_left[m.lora_left_mask].any()) and bool(m.lora_left[~m.lora_left_mask].all())
+
+
+def test_transposed_codes_follow_the_codes_and_can_be_given_back():
+    from slim_amd.packed import Int8Linear
+    torch.manual_seed(0)
+    m = Int8Linear(torch.nn.Linear(300, 200, bias=False).to(DEV))
+    x, dy = torch.randn(7, 300, device=DEV, requires_grad=True), torch.randn(7, 200, device=DEV)
+
+    def check():
+        (dx,) = torch.autograd.grad(m(x), [x], dy)
+        exact = dy.double() @ m.dense_weight().double()
+        # sums of 200 fp32 products (each rounded, and the weight's too): 2^-23 for each at most
+        size = dy.double().abs() @ m.dense_weight().double().abs()
+        assert bool(((dx.double() - exact).abs() <= 210 * 2.0 ** -23 * size).all())
+    check()
+    kept = m.transposed()
+    assert m.transposed() is kept
+    m.codes.neg_()                                            # changed in place
+    check()
+    m.codes = m.codes.flip(0).contiguous()                    # replaced
+    check()
+    del kept
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    m.drop_transposed()
+    assert before - torch.cuda.memory_allocated() >= 300 * 256
+    check()
+    with torch.inference_mode():
+        n = Int8Linear(torch.nn.Linear(300, 200, bias=False).to(DEV))
+    m.codes, m.scale = n.codes, n.scale
+    check()
