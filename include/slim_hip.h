@@ -544,7 +544,8 @@ int slim_linear24_forward_q4(const void* x_bf16, int64_t ldx, int64_t M, int64_t
 int64_t slim_rows8_ld(int64_t K);
 /* codes[r][k] = rint(x[r][k] * (127 / a)), scale[r] = a / 127, a = max |x[r][:]| (fp32 operations, each rounded once).  A row
  * with a < 2^-100 gets scale 0 and zero codes; a row that holds an infinity or a NaN gets the scale NaN and zero codes.  x: rows
- * of ldx >= K elements at any element-aligned address; codes 16-byte aligned, ldc >= slim_rows8_ld(K) and a multiple of 16. */
+ * of ldx >= K elements at any element-aligned address; codes 16-byte aligned, ldc >= slim_rows8_ld(K) and a multiple of 16.  At most 2^24 - 1
+ * rows, 2^22 - 2 of them where K > 16384 (in the linears as well). */
 int slim_quantize_rows8(const void* x, int dtype, int64_t R, int64_t K, int64_t ldx, int8_t* codes, int64_t ldc, float* scale, void* stream);
 /* codes_t[k][n] = codes[n][k] for n < N, 0 up to ldt >= slim_rows8_ld(N): the operand of slim_linear8_backward. */
 int slim_transpose8(const int8_t* codes, int64_t N, int64_t K, int64_t ld, int8_t* codes_t, int64_t ldt, void* stream);

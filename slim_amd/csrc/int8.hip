@@ -107,9 +107,11 @@ __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void quantize_rows_kernel(c
 template <typename T>
 int quantize_rows(const T* x, int64_t R, int64_t K, int64_t ldx, int8_t* codes, int64_t ldc, float* scale, hipStream_t st) {
     const int64_t pieces = (K + 127) / 128 * 16;         // pieces of eight codes in a padded row
-    SLIM_REQUIRE(R * (pieces > 1024 ? 1024 : 256) < (int64_t)1 << 32, "quantize_rows8: too many rows for one launch");
 #define SLIM_ROWS(NV, WPR)                                                                                                  \
-    quantize_rows_kernel<T, NV, WPR><<<(unsigned)(WPR > 1 ? R : ceil_div64(R, 4)), WPR == 16 ? 1024 : 256, 0, st>>>(x, R, K, ldx, codes, ldc, scale)
+    do {                                                                                                                    \
+        SLIM_REQUIRE(R * 64 * WPR < ((int64_t)1 << 32) - 1024, "slim_quantize_rows8: too many rows of this length for one launch"); \
+        quantize_rows_kernel<T, NV, WPR><<<(unsigned)(WPR > 1 ? R : ceil_div64(R, 4)), WPR == 16 ? 1024 : 256, 0, st>>>(x, R, K, ldx, codes, ldc, scale); \
+    } while (0)
     if (pieces <= 64) SLIM_ROWS(1, 1);
     else if (pieces <= 128) SLIM_ROWS(2, 1);
     else if (pieces <= 256) SLIM_ROWS(4, 1);

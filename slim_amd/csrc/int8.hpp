@@ -100,5 +100,5 @@ struct Columns {
 
 // the longest reduction whose sums of products of codes in [-128, 127] fit 32 bits
 #define SLIM_INT8_MAX_REDUCTION 131071
-// rows and columns: a workgroup of 256 threads each stays below a grid's 2^32 threads
+// rows and columns: a workgroup of 256 threads each stays below a grid's 2^32 threads (long rows take 1024: 2^22 - 1 of more than 16384 elements)
 #define SLIM_INT8_MAX_DIM ((1 << 24) - 1)
