@@ -73,3 +73,33 @@ def test_hooks_of_the_linear_carry_over(layer):
     other = Int8Linear.from_tensors(dict(codes=layer.codes, scale=layer.scale), N, K, "cpu")
     other._take_hooks(plain)                                 # an input quantiser and the mask of a trained weight: neither is called
     assert torch.equal(other(x), before) and len(plain._forward_pre_hooks) == 2 and not other._forward_pre_hooks
+
+
+def decoder(*linears):
+    model = torch.nn.Module()
+    model.model = torch.nn.Module()
+    model.model.layers = torch.nn.ModuleList([torch.nn.Sequential(*linears)])
+    return model
+
+
+def test_files_hold_one_known_kind(layer, tmp_path):
+    """A model of both kinds is not saved, a file of another format not loaded; the kind that a file names is what it becomes."""
+    from safetensors.torch import save_file
+    from slim_amd.packed import PackedLinear, load_packed, save_packed
+    mixed = PackedLinear()
+    mixed.sf = torch.ones(1)
+    mixed.vals = mixed.meta = torch.zeros(8, dtype=torch.uint8)
+    mixed.bias = mixed.LeffT = mixed.ReffT = mixed.qL = mixed.qR = None
+    mixed.out_features, mixed.in_features, mixed.rank, mixed.a_div, mixed.qblock = 2, 16, 0, 1.0, 0
+    with pytest.raises(ValueError, match="one kind"):
+        save_packed(decoder(layer, mixed), str(tmp_path / "both"))
+    assert not (tmp_path / "both").exists()
+    save_file({"0.0.codes": layer.codes}, str(tmp_path / "foreign"), metadata={"format": "another/1", "layers": "{}"})
+    with pytest.raises(ValueError, match="not a"):
+        load_packed(decoder(torch.nn.Linear(K, N)), str(tmp_path / "foreign"), device="cpu")
+    save_packed(decoder(layer), str(tmp_path / "int8"))
+    model = decoder(torch.nn.Linear(K, N))
+    assert load_packed(model, str(tmp_path / "int8"), device="cpu") == 1
+    loaded = model.model.layers[0][0]
+    x = torch.randn(3, K)
+    assert isinstance(loaded, Int8Linear) and torch.equal(loaded.codes, layer.codes) and torch.equal(loaded(x), layer(x))
