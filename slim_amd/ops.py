@@ -1133,11 +1133,11 @@ def _operand(t, dtype, index, name):
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _codes8(t, index, name):
-    """A contiguous int8 matrix of codes and its shape."""
+def _codes8(t, index, name, empty=False):
+    """A contiguous int8 matrix of codes and its shape; without rows only where `empty`."""
     t = _operand(t, torch.int8, index, name)
     shape = t.shape
-    if len(shape) != 2 or shape[0] == 0 or shape[1] == 0 or shape[1] % 128:
+    if len(shape) != 2 or shape[0] == 0 and not empty or shape[1] == 0 or shape[1] % 128:
         raise ValueError(f"{name} must be [rows, a multiple of 128], got {tuple(shape)}")
     return t, shape[0], shape[1]
 
@@ -1200,7 +1200,7 @@ def gemm8_nt(a, sa, b, sb, bias=None, out_dtype=BF16, K=None):
     quantize_rows8 makes them: the sum in whole numbers, the rest in fp32, rounded once to out_dtype.  K: the number of columns
     that are not padding (all when None), at most 131071."""
     gpu = _gpu_of(a, "a")
-    a, M, Kp = _codes8(a, gpu, "a")
+    a, M, Kp = _codes8(a, gpu, "a", empty=True)
     b, N, Kb = _codes8(b, gpu, "b")
     if Kb != Kp:
         raise ValueError(f"a and b must have equally long rows, got {Kp} and {Kb}")
@@ -1213,6 +1213,8 @@ def gemm8_nt(a, sa, b, sb, bias=None, out_dtype=BF16, K=None):
     if bias is not None:
         bias = _vector(bias, N, out_dtype, gpu, "bias")
     out = _matrix(M, N, out_dtype, a.device)
+    if not M:
+        return out
     need = _lib.query("slim_gemm8_workspace_bytes", M, N, K)
     ws = _workspace(need, a.device)
     _call_at(gpu, "slim_gemm8_nt", a.data_ptr(), Kp, sa.data_ptr(), b.data_ptr(), Kp, sb.data_ptr(), M, N, K, _p(bias), _DTYPES[out_dtype], out.data_ptr(), N,

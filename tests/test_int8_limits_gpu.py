@@ -1,4 +1,4 @@
-"""The largest numbers of rows of the 8-bit linears."""
+"""The largest and smallest numbers of rows of the 8-bit linears."""
 import pytest
 import torch
 
@@ -28,3 +28,19 @@ def test_more_than_four_million_long_rows():
     few, few_scale = ops.quantize_rows8(x[-3:].clone())
     assert torch.equal(codes[-3:], few) and torch.equal(scale[-3:], few_scale) and bool(few.any())
     assert not bool(scale[:-3].any()) and not bool(codes[:5].any()) and not bool(codes[-8:-3].any())
+
+
+@pytest.mark.gpu
+def test_no_rows_at_all():
+    """An empty batch through the parts, as through the whole: quantised, multiplied and sent back."""
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    from slim_amd import ops
+    codes, scale = ops.quantize_rows8(torch.randn(10, 100, device=DEV))
+    a, sa = ops.quantize_rows8(torch.zeros(0, 100, device=DEV))
+    out = ops.gemm8_nt(a, sa, codes, scale, torch.zeros(10, device=DEV), torch.float32, K=100)
+    assert out.shape == (0, 10) and out.dtype == torch.float32
+    assert ops.linear8_forward(torch.zeros(0, 100, device=DEV), codes, scale).shape == (0, 10)
+    assert ops.linear8_backward(torch.zeros(0, 10, device=DEV), ops.transpose8(codes, 100), scale).shape == (0, 100)
+    with pytest.raises(ValueError, match="b must be"):
+        ops.gemm8_nt(codes, scale, a, sa)
