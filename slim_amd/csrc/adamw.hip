@@ -192,7 +192,9 @@ int64_t chunks_of(int64_t n) { return ceil_div64(n, CHUNK); }
 int64_t norm_chunks_of(int64_t n) { return ceil_div64(n, NORM_CHUNK); }
 
 // ---- the update -----------------------------------------------------------------------------------------------------
-// a 32-bit mix of position and key (multiply and xor-shift, twice); its halves are the random numbers of the two moments
+// a 32-bit mix of position and key, the published integer hash lowbias32 (C. Wellons, 2018: xor-shifts by 16, 15 and 16 around two odd
+// factors) over a Weyl sequence; its halves are the random numbers of the two moments.  (The keys' odd factors are those that the
+// MurmurHash3 and xxHash mixes use; any odd numbers with as many bits would do.)
 __device__ __forceinline__ uint32_t mix(uint32_t i, uint32_t key) {
     uint32_t h = i * 0x9e3779b9u + key;
     h ^= h >> 16;

@@ -27,7 +27,7 @@ __device__ __forceinline__ uint2 encode(const float x[8], float r) {
 }
 
 // WPR waves work on a row (one: four rows per workgroup; four or sixteen: one); each thread keeps NV pieces of eight elements in registers, so
-// the row is read once, with loads that do not stay in the caches (28672 x 8192 bf16: 109 us, 6.4 TB/s; 126 without).
+// the row is read once, with loads that do not stay in the caches (28672 x 8192 bf16: 111 us, 6.3 TB/s; 127 without).
 // NV = 0: rows too long for that are read twice.
 template <typename T, int NV, int WPR>
 __global__ __launch_bounds__(WPR == 16 ? 1024 : 256) void quantize_rows_kernel(const T* __restrict__ x, int64_t R, int64_t K, int64_t ldx,
@@ -204,10 +204,10 @@ __device__ __forceinline__ void write_results(const Gemm8Args& g, const i32x4 (&
 // Fragments are double-buffered in registers: while a step's first half (64 bytes) is multiplied its second half is read, and
 // while that is multiplied the next step's first half is read and the stage just emptied is requested again -- one read or request
 // per two matrix instructions, one barrier per step.  Left to the compiler the reads come in a burst that the matrix instructions
-// wait for (4096 x 11008 x 4096, 256 x 256 tile: 185 us against 159; 8192^3: 485 against 397 us, 2.8e15 operations/s).
-// Whole 128-byte lines per row: with 64-byte steps, which would allow four stages, the requests take twice as long (171 us).
-// What bounds it: without requests the loop takes 138 us, without fragment reads as well 123 us; the matrix instructions alone hold
-// the clock at about 2.1 GHz.
+// wait for (4096 x 11008 x 4096 on 256 x 256 tiles: 176 us against 169; 8192^3: 404 against 393 us, 2.8e15 operations/s).
+// Whole 128-byte lines per row: with 64-byte steps, which would allow four stages, the requests take twice as long (8 % of the whole).
+// What bounds it: without requests the loop takes 87 % of its time, without fragment reads as well 77 %; the matrix instructions alone
+// hold the clock at about 2.1 GHz.
 template <int FM, int FN, int WM, int WN, int STAGES>
 __device__ __forceinline__ void gemm8_tile(const Gemm8Args& g, char* lds, int64_t row0, int64_t col0, int slice) {
     constexpr int BM = 16 * FM * WM, BN = 16 * FN * WN, NW = WM * WN;
@@ -343,8 +343,8 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void gemm8_kernel(const Gemm8Arg
 
 // The same product by workgroups that stay, for more tiles than CUs: each takes every gridDim.x-th tile, and the stream of requests
 // runs on from one tile into the next, so that the next tile's first steps travel while the finished one is scaled and stored, and its
-// stores drain under the next tile's products (a workgroup a tile: 4096 x 11008 x 4096 164 us, 159 so; 8192^3 399 and 382, 8192 x 4096 x
-// 1024 47 and 41).  REST > 0: behind the columns of full tiles lie g.rest_n columns of tiles of 16 REST WN columns, which fill the last
+// stores drain under the next tile's products (us, a workgroup a tile / so: 4096 x 11008 x 4096 169 / 164, 8192^3 393 / 382, 8192 x 4096 x
+// 1024 43 / 38).  REST > 0: behind the columns of full tiles lie g.rest_n columns of tiles of 16 REST WN columns, which fill the last
 // round of workgroups better.  The scales of a tile come by LDS-DMA while it is multiplied.  (g.steps >= 2)
 template <int FM, int FN, int WM, int WN, int REST>
 __global__ __launch_bounds__(64 * WM * WN, 2) void gemm8_stream_kernel(const Gemm8Args g) {
@@ -573,7 +573,7 @@ Plan plan_gemm8(int64_t M, int64_t N, int64_t steps) {
         }
     }
     // The largest tile's last round, when it is not full, on narrower tiles that fill it better (4096 x 11008: 512 full tiles and 240 of
-    // 192 columns in place of 176 full ones).
+    // 192 columns in place of 176 full ones: reduction 4096 150 us, full tiles 153; 2048 x 11008 88 and 96).
     if (best.tile == 0 && best.splits == 1 && best.steps_per_split >= 2 && best.tiles_m <= 256) {
         const int64_t count = best.tiles_m * best.tiles_n, columns = count / 256 * 256 / best.tiles_m;
         if (count > 256 && count % 256 && columns < best.tiles_n) {

@@ -111,3 +111,91 @@ def test_gradient_is_that_of_differences_of_the_dense_product(ops):
         e[k] = 0.5
         quotient = loss(x + e) - loss(x - e)
         assert bool(((quotient - dx[:, k]).abs() <= allowed[:, k] + 1e-9).all())
+
+
+def close(ops, dx, dy, wt, scale, N, rows, cols=slice(None)):
+    """Rows and columns of a gradient against 64 bits, within the header's bound."""
+    w = wt[cols, :N].t()
+    exact, allowed = documented(dy[rows].double() * scale.double(), w, dy.dtype)
+    return bool(((dx[rows][:, cols].double() - exact).abs() <= allowed).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,K", [(700, 300), (1500, 300)])
+def test_gradients_of_views(ops, N, K, dtype):
+    """Rows that start at odd elements, rows and columns apart, one row for all (what a sum sends back), transposed; one launch and two."""
+    w, wt = half_zero_codes(ops, N, K, 8)
+    scale = torch.rand(N, device=DEV) * 1e-2
+    big = torch.randn(60, 2 * N + 9, device=DEV).to(dtype)
+    for dy in (big[3:40, 1:N + 1], big[::3, 7:N + 7], big[:, :2 * N:2], big[5:6, 2:N + 2], big[1:2, :N].expand(33, N), big.t()[:N].t(), big[:N, :40].t()[:, :1].expand(40, N)):
+        assert dy.shape[1] == N and close(ops, ops.linear8_backward(dy, wt, scale), dy, wt, scale, N, slice(None))
+
+
+@pytest.mark.parametrize("M,N,K", [(19, 200, 70), (19, 1200, 70), (300, 1300, 2101), (2000, 1100, 5003)])
+def test_gradient_rows_apart_and_what_lies_between(ops, M, N, K):
+    """Through the C entry: results at an odd element, rows apart; nothing beside them is written."""
+    from slim_amd import _lib
+    w, wt = half_zero_codes(ops, N, K, 9)
+    scale, dy = torch.rand(N, device=DEV) * 1e-2, torch.randn(M, N, device=DEV).bfloat16()
+    ld = K + 29
+    out = torch.full((M * ld + 40,), 7.0, device=DEV, dtype=torch.bfloat16)
+    need = _lib.query("slim_linear8_backward_workspace_bytes", M, N, K, 1)
+    ws = torch.full((need + 256,), 85, dtype=torch.uint8, device=DEV)
+    _lib.call("slim_linear8_backward", dy.data_ptr(), 1, N, M, N, wt.data_ptr(), scale.data_ptr(), K, out.data_ptr() + 2, ld, ws.data_ptr() if need else None, need,
+              torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(torch.as_strided(out, (M, K), (ld, 1), 1), ops.linear8_backward(dy, wt, scale))
+    torch.as_strided(out, (M, K), (ld, 1), 1).fill_(7.0)
+    assert bool((out == 7.0).all()) and bool((ws[need:] == 85).all())
+
+
+@pytest.mark.parametrize("M,N,K", [(40, 300, 500), (40, 1500, 500), (400, 1200, 2500), (1500, 2000, 4000)])
+def test_captured_and_on_several_streams(ops, M, N, K):
+    w, wt = half_zero_codes(ops, N, K, 10)
+    scale = torch.rand(N, device=DEV) * 1e-2
+    dy = torch.randn(M, N, device=DEV).bfloat16()
+    ops.linear8_backward(dy, wt, scale)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):                                      # (two graphs that live at once, each with its workspace)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            dx = ops.linear8_backward(dy, wt, scale)
+        graphs.append((graph, dx))
+    for i in range(4):
+        dy.copy_(torch.randn(M, N, device=DEV) * 10.0 ** i)
+        for graph, _ in graphs:
+            graph.replay()
+        ops.linear8_backward(torch.randn(M + 5, N, device=DEV), wt, scale)
+        torch.cuda.synchronize()
+        want = ops.linear8_backward(dy, wt, scale)
+        assert all(torch.equal(dx, want) for _, dx in graphs)
+    streams, outs = [torch.cuda.Stream() for _ in range(3)], []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(ops.linear8_backward(dy, wt, scale))
+    torch.cuda.synchronize()
+    assert all(torch.equal(dx, want) for dx in outs)
+
+
+def test_gradient_offsets_beyond_32_bits(ops):
+    """A result, the planes of the rows, and transposed codes of more than 2^31 elements each."""
+    for M, N, K in ((70001, 1100, 32000), (1000001, 2048, 24)):
+        w, wt = half_zero_codes(ops, N, K, 11)
+        scale, dy = torch.rand(N, device=DEV) * 1e-2, torch.randn(M, N, device=DEV, dtype=torch.bfloat16)
+        dx = ops.linear8_backward(dy, wt, scale)
+        assert M * K > 2 ** 31 or 2 * M * N > 2 ** 31
+        assert close(ops, dx, dy, wt, scale, N, [0, 1, M // 2, M - 17, M - 1])
+        del dx, dy, w, wt
+    N, K = 131071, 17001
+    wt = torch.randint(-127, 128, (K, 131072), dtype=torch.int8, device=DEV)
+    wt[:, N:] = 0
+    scale = torch.rand(N, device=DEV) * 1e-2
+    assert wt.numel() > 2 ** 31
+    for dtype, M in ((torch.bfloat16, 5), (torch.float32, 300)):
+        dy = torch.randn(M, N, device=DEV).to(dtype)
+        dx = ops.linear8_backward(dy, wt, scale)
+        for cols in (slice(0, 300), slice(K - 300, K)):
+            assert close(ops, dx, dy, wt, scale, N, [0, M - 1], cols)
