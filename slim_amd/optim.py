@@ -29,6 +29,16 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, master_weights=False,
                  max_grad_norm=None, seed=0):
+        self._check_options(dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+        if max_grad_norm is not None and not max_grad_norm > 0:
+            raise ValueError(f"max_grad_norm must be positive, got {max_grad_norm}")
+        self.max_grad_norm = max_grad_norm
+        self.last_norm = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, master_weights=master_weights, seed=int(seed)))
+
+    @staticmethod
+    def _check_options(group):
+        lr, eps, weight_decay, betas, state_bits = (group[k] for k in ("lr", "eps", "weight_decay", "betas", "state_bits"))
         if not lr >= 0 or not eps >= 0 or not weight_decay >= 0:
             raise ValueError(f"lr, eps and weight_decay must not be negative, got {lr}, {eps}, {weight_decay}")
         if 0 < eps < 2.0 ** -126:
@@ -37,11 +47,11 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"betas must lie in [0, 1), got {betas}")
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
-        if max_grad_norm is not None and not max_grad_norm > 0:
-            raise ValueError(f"max_grad_norm must be positive, got {max_grad_norm}")
-        self.max_grad_norm = max_grad_norm
-        self.last_norm = None
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, master_weights=master_weights, seed=int(seed)))
+
+    def add_param_group(self, param_group):
+        """torch's, with the checks of the constructor on a group's own options."""
+        self._check_options({**self.defaults, **param_group})
+        super().add_param_group(param_group)
 
     @property
     def seed(self):

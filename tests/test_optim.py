@@ -75,3 +75,16 @@ def test_the_seed_is_saved():
     opt = AdamW([parameter(dtype=torch.float32)], seed=8)
     opt.load_state_dict(torch.optim.AdamW([q]).state_dict())               # (which has none)
     assert [g["seed"] for g in opt.param_groups] == [8]
+
+
+@pytest.mark.parametrize("option", [dict(state_bits=16), dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=2.0 ** -130), dict(weight_decay=-0.1)])
+def test_a_groups_own_options_are_checked(option):
+    """As the constructor's are: 16-bit moments were taken for 32-bit ones."""
+    with pytest.raises(ValueError):
+        AdamW([dict(params=[parameter()], **option)])
+    opt = AdamW([parameter()])
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=[parameter()], **option))
+    assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=[parameter()], state_bits=8))
+    assert opt.param_groups[1]["state_bits"] == 8
